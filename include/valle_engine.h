@@ -371,6 +371,52 @@ int vle_op_topk_sample(void* stream, const float* logits, int64_t rows, int32_t 
 int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float* be, float* gamma_out, float* beta_out,
                       int32_t d);
 
+/* ---- attention with a window, and a paged key-value cache -------------------------------------------------------------------
+ * A cache that stays bounded over long utterances: rows see a sliding window, the first `sinks` tokens and the text prefix; the keys
+ * live in pages that any sequence can own; keys that got little attention leave.  The prefix-LM mask of vle_op_attention
+ * (valle/models/valle.py:1019-1033) is the case window = 0 of the first.
+ *   row i of a sequence sees key j  iff  j < text_len  or  (j <= i and (window == 0 or i - j < window or j < sinks))
+ * dtype VLE_DTYPE_F32 / _BF16 (T); head size a multiple of 8, <= 128; nhead a multiple of nhead_kv (query head h reads key-value head
+ * h / (nhead / nhead_kv)), at most 256 per key-value head; strides in elements, every row and head on 16 bytes; scale > 0
+ * (1 / sqrt(dh) as a rule).  All pointers DEVICE, index arrays int32.  A bad argument is refused with VLE_EINVAL before any launch;
+ * what index arrays hold is bounded inside the kernels: offsets and lengths are clamped to the rows / the table, and a page id outside
+ * [0, n_pages) is never followed -- its keys are absent.  The HIP device current at the call must be the stream's.
+ * Nothing is allocated and nothing waits: every call can be captured into a graph.
+ *
+ * vle_op_window_attention: packed sequences, rows seq_off[b] .. seq_off[b + 1] - 1 of q / k / v [rows][heads][dh]; out T [rows][nhead][dh].
+ *   Rows that no sequence holds are left as they were, or set to 0 where zero_rest != 0.  text_len may be NULL (0).
+ * vle_op_paged_kv_write: row r of sequence b (seq_off as above, or NULL: row b alone) becomes key start[b] + r - seq_off[b], in slot
+ *   pos % page_size of page page_table[b][pos / page_size] of k_pages / v_pages T [n_pages][nhead_kv][page_size][dh]; its mass (NULL or f32
+ *   [n_pages][nhead_kv][page_size]) becomes 0.  Positions past the table are dropped.  page_size: a power of two, >= 8.
+ * vle_op_paged_decode_attention: q T [B][nhead][dh], the newest token of sequence b is key lengths[b] - 1; out T [B][nhead][dh] (0 where no
+ *   key is visible).  mass != NULL: += the weight every visible key received, summed over the query heads of its key-value head.
+ *   Sequences may share pages (their weights are then added in no fixed order).  workspace: vle_op_paged_decode_workspace_bytes(...) bytes
+ *   (may be 0) on 16 bytes, not used by another call at the same time.
+ * vle_op_kv_evict: sequences of more than `budget` keys keep the first max(text_len, sinks), the last `recent` and, of those between, the
+ *   keys with the largest mass (of equal ones the earlier; NaN counts as the largest), per key-value head, `budget` in all; text_len beyond the
+ *   budget takes all of it, and what it leaves bounds `recent`.  The keys that stay move up in order, in place, with their mass.
+ *   kept int32 [B][nhead_kv][budget]: their old positions, ascending (-1 past the end); new_lengths int32 [B] = min(lengths, budget).
+ *   A page belongs to one sequence here. */
+int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                            int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
+                            const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,
+                            int32_t window, int32_t sinks, float scale, int32_t zero_rest);
+int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                          int64_t v_head, void* k_pages, void* v_pages, float* mass, const int32_t* page_table_dev,
+                          const int32_t* start_dev, const int32_t* seq_off_dev, int64_t rows, int32_t B, int32_t nhead_kv, int32_t dh,
+                          int32_t n_pages, int32_t table_width, int32_t page_size);
+int64_t vle_op_paged_decode_workspace_bytes(int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
+                                            int32_t page_size, int32_t window, int32_t sinks, int32_t has_text, int32_t has_mass);
+int vle_op_paged_decode_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
+                                  const void* v_pages, const int32_t* page_table_dev, const int32_t* lengths_dev,
+                                  const int32_t* text_len_dev, float* mass, void* workspace, int64_t workspace_bytes, void* out,
+                                  int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t n_pages, int32_t table_width,
+                                  int32_t page_size, int32_t window, int32_t sinks, float scale);
+int vle_op_kv_evict(void* stream, int dtype, void* k_pages, void* v_pages, float* mass, const int32_t* page_table_dev,
+                    const int32_t* lengths_dev, const int32_t* text_len_dev, int32_t* kept, int32_t* new_lengths, int32_t B,
+                    int32_t nhead_kv, int32_t dh, int32_t n_pages, int32_t table_width, int32_t page_size, int32_t budget,
+                    int32_t recent, int32_t sinks);
+
 /* ---- EnCodec 24 kHz decoder: codes -> waveform --------------------------------------------------
  * Replaces audio_tokenizer.decode([(codes.transpose(2, 1), None)]) (valle/bin/infer.py:261-263; AudioTokenizer.decode ->
  * EncodecModel.decode, valle/data/tokenizer.py:241-242; third-party `encodec`, encodec_model_24khz at 6 kbps = 8 codebooks).

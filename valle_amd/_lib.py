@@ -81,6 +81,14 @@ SIGNATURES = {
     "vle_op_cross_entropy": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
     "vle_op_cross_attention": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "vle_op_topk_sample": (C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_uint64, C.c_uint32, _P, _P]),
+    "vle_op_window_attention": (C.c_int, [_P, C.c_int, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, _P, _P,
+                                          C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float, C.c_int32]),
+    "vle_op_paged_kv_write": (C.c_int, [_P, C.c_int, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64,
+                                        C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "vle_op_paged_decode_workspace_bytes": (C.c_int64, [C.c_int32] * 10),
+    "vle_op_paged_decode_attention": (C.c_int, [_P, C.c_int, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P] + [C.c_int32] * 9
+                                      + [C.c_float]),
+    "vle_op_kv_evict": (C.c_int, [_P, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P] + [C.c_int32] * 9),
     "vle_op_adaln_fold": (C.c_int, [_P, _P, _P, _P, _P, _P, C.c_int32]),
 }
 

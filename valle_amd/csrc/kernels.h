@@ -477,4 +477,61 @@ int launch_check_ids(hipStream_t st, int64_t* ids, int64_t stride0, int row_stri
 int launch_codes_set_first(hipStream_t st, const int64_t* first_cb, int64_t fc_stride, const int32_t* grow_seq,
                            const int32_t* grow_pos, int64_t rows, int64_t* codes, int64_t g_stride, int Q);
 
+// ---- window_attn.hip --------------------------------------------------------------------------
+// Prompt attention over packed sequences, grouped heads: row i of a sequence sees key j iff j < text_len or (j <= i and (window <= 0 or
+// i - j < window or j < sinks)).  Strides in elements; every row and head starts on 16 bytes.
+struct WindowAttnArgs {
+  const void *q, *k, *v;
+  void* out;  // [rows][H][dh], contiguous
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t* seq_off;   // [B + 1]
+  const int32_t* text_len;  // [B] or null
+  int64_t rows;
+  int B, H, Hkv, dh, window, sinks, zero_rest;  // zero_rest: rows no sequence holds are set to 0 instead of left as they are
+  float sl2;                                    // scale * log2(e)
+};
+int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a);
+
+// ---- paged_cache.hip --------------------------------------------------------------------------
+struct PagedWriteArgs {
+  const void *k, *v;  // T [rows][Hkv][dh], strided
+  int64_t k_row, k_head, v_row, v_head;
+  void *k_pages, *v_pages;  // T [n_pages][Hkv][1 << psl][dh]
+  float* mass;              // [n_pages][Hkv][1 << psl] or null: set to 0 where a key is written
+  const int32_t *table, *start, *seq_off;  // seq_off null: one row per sequence
+  int64_t rows;
+  int B, Hkv, dh, n_pages, W, psl;
+};
+int launch_paged_write(hipStream_t st, int dtype, const PagedWriteArgs& a);
+
+struct PagedDecodeArgs {
+  const void* q;  // T [B][H][dh], strided
+  int64_t q_b, q_h;
+  const void *k_pages, *v_pages;
+  void* out;    // T [B][H][dh], contiguous
+  float* mass;  // or null
+  const int32_t *table, *lengths, *text_len;  // text_len may be null
+  float *part_o, *part_ml, *scores;           // workspace (paged_decode_plan)
+  int Hkv, G, dh, n_pages, W, psl, window, sinks;
+  float sl2;
+  // set by the launcher
+  int GT, chunk, nsplit;
+  int64_t score_ld;
+};
+struct PagedDecodePlan {  // split of the cache's length, and the workspace it needs
+  int tiles, chunk, nsplit, nw;
+  size_t ml_floats, o_floats, score_floats;
+};
+PagedDecodePlan paged_decode_plan(int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass);
+int launch_paged_decode(hipStream_t st, int dtype, const PagedDecodePlan& p, PagedDecodeArgs a, int B);
+
+struct EvictArgs {
+  void *k_pages, *v_pages;
+  float* mass;
+  const int32_t *table, *lengths, *text_len;
+  int32_t *kept, *new_lengths;  // [B][Hkv][budget], [B]
+  int Hkv, n_pages, W, psl, budget, recent, sinks;
+};
+int launch_kv_evict(hipStream_t st, int dtype, const EvictArgs& a, int B, int dh);
+
 }  // namespace vle

@@ -1,5 +1,6 @@
 // C ABI of the stand-alone Transformer-block operators (valle_engine.h, "operator surface"):
 // thin argument checks around the kernel launchers, no engine instance needed.
+#include <cstdio>
 #include <string>
 
 #include "common.h"
@@ -279,4 +280,138 @@ extern "C" int vle_op_linear_fp8(void* stream, const void* a8, const float* a_sc
   const int r = launch_gemm_fp8((hipStream_t)stream, a8, a_scale, w8, w_scale, bias, out, resid, M, N, K, epilogue);
   if (r == 1) return op_fail("vle_op_linear_fp8: shape not covered (K % 128, N % 4)");
   return op_done(r, "vle_op_linear_fp8");
+}
+
+// ---- attention with a window, and the paged key-value cache ----------------------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static bool vec_strides(int dtype, int64_t row, int64_t head) {  // every row and head starts on 16 bytes
+  const int64_t v = dtype == DT_F32 ? 4 : 8;
+  return row >= 0 && head >= 0 && row % v == 0 && head % v == 0;
+}
+static const char* heads_fault(int dtype, int32_t nhead, int32_t nhead_kv, int32_t dh) {
+  if (dtype != DT_F32 && dtype != DT_BF16) return "dtype must be f32 or bf16";
+  if (nhead < 1 || nhead_kv < 1 || nhead % nhead_kv) return "nhead must be a multiple of nhead_kv";
+  if (nhead / nhead_kv > 256) return "at most 256 query heads share a key-value head";
+  if (dh < 8 || dh > 128 || dh % 8) return "head size must be a multiple of 8 up to 128";
+  return nullptr;
+}
+static const char* cache_fault(int32_t B, int32_t nhead_kv, int32_t dh, int32_t n_pages, int32_t table_width, int32_t page_size) {
+  if (B < 0 || B > 65535) return "0 to 65535 sequences";
+  if (nhead_kv > 4096) return "at most 4096 key-value heads";
+  if (n_pages < 1 || table_width < 1) return "no pages";
+  if (page_size < 8 || (page_size & (page_size - 1))) return "page size must be a power of two, 8 at least";
+  if ((int64_t)table_width * page_size > 0x3fffffff) return "a sequence holds fewer than 2^30 keys";
+  if ((int64_t)nhead_kv * page_size * dh > 0x3fffffff) return "a page holds fewer than 2^30 elements";
+  return nullptr;
+}
+static int log2_of(int32_t v) { return 31 - __builtin_clz((unsigned)v); }
+static int op_refuse(const char* op, const char* why) {
+  char msg[192];
+  snprintf(msg, sizeof msg, "%s: %s", op, why);
+  return op_fail(msg);
+}
+
+extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                                       int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
+                                       const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,
+                                       int32_t window, int32_t sinks, float scale, int32_t zero_rest) {
+  const char* op = "vle_op_window_attention";
+  if (const char* e = heads_fault(dtype, nhead, nhead_kv, dh)) return op_refuse(op, e);
+  if (rows < 0 || rows > 0x7fff0000 || B < 0) return op_refuse(op, "bad number of rows or sequences");
+  if (window < 0 || sinks < 0) return op_refuse(op, "window and sinks must not be negative");
+  if (!(scale > 0.f) || scale > 3.0e38f) return op_refuse(op, "scale must be positive and finite");
+  if (rows == 0) return VLE_OK;
+  if (!q || !k || !v || !out || !seq_off_dev) return op_refuse(op, "null operand");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !vec_strides(dtype, q_row, q_head) ||
+      !vec_strides(dtype, k_row, k_head) || !vec_strides(dtype, v_row, v_head))
+    return op_refuse(op, "rows and heads must start on 16 bytes");
+  WindowAttnArgs a;
+  a.q = q; a.k = k; a.v = v; a.out = out;
+  a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+  a.seq_off = seq_off_dev; a.text_len = text_len_dev; a.rows = rows; a.B = B; a.H = nhead; a.Hkv = nhead_kv; a.dh = dh;
+  a.window = window; a.sinks = sinks; a.zero_rest = zero_rest;
+  a.sl2 = scale * 1.4426950408889634f;
+  const int r = launch_window_attention((hipStream_t)stream, dtype, a);
+  if (r == -1) return op_refuse(op, "too many rows times heads for one launch");
+  return op_done(r, op);
+}
+
+extern "C" int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                                     int64_t v_head, void* k_pages, void* v_pages, float* mass, const int32_t* page_table_dev,
+                                     const int32_t* start_dev, const int32_t* seq_off_dev, int64_t rows, int32_t B, int32_t nhead_kv, int32_t dh,
+                                     int32_t n_pages, int32_t table_width, int32_t page_size) {
+  const char* op = "vle_op_paged_kv_write";
+  if (const char* e = heads_fault(dtype, nhead_kv, nhead_kv, dh)) return op_refuse(op, e);
+  if (const char* e = cache_fault(B, nhead_kv, dh, n_pages, table_width, page_size)) return op_refuse(op, e);
+  if (rows < 0 || rows > 0x7fff0000 || (!seq_off_dev && rows != B)) return op_refuse(op, "without seq_off there is one row per sequence");
+  if (rows == 0 || B == 0) return VLE_OK;
+  if (!k || !v || !k_pages || !v_pages || !page_table_dev || !start_dev) return op_refuse(op, "null operand");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || !vec_strides(dtype, k_row, k_head) ||
+      !vec_strides(dtype, v_row, v_head))
+    return op_refuse(op, "rows and heads must start on 16 bytes");
+  PagedWriteArgs a;
+  a.k = k; a.v = v; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+  a.k_pages = k_pages; a.v_pages = v_pages; a.mass = mass; a.table = page_table_dev; a.start = start_dev; a.seq_off = seq_off_dev;
+  a.rows = rows; a.B = B; a.Hkv = nhead_kv; a.dh = dh; a.n_pages = n_pages; a.W = table_width; a.psl = log2_of(page_size);
+  return op_done(launch_paged_write((hipStream_t)stream, dtype, a), op);
+}
+
+extern "C" int64_t vle_op_paged_decode_workspace_bytes(int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
+                                                       int32_t page_size, int32_t window, int32_t sinks, int32_t has_text, int32_t has_mass) {
+  const char* op = "vle_op_paged_decode_workspace_bytes";
+  const char* e = heads_fault(DT_F32, nhead, nhead_kv, dh);
+  if (!e) e = cache_fault(B, nhead_kv, dh, 1, table_width, page_size);
+  if (!e && (window < 0 || sinks < 0)) e = "window and sinks must not be negative";
+  if (e) return op_refuse(op, e);
+  const PagedDecodePlan p = paged_decode_plan(B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, has_text != 0, has_mass != 0);
+  return (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
+}
+
+extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
+                                             const void* v_pages, const int32_t* page_table_dev, const int32_t* lengths_dev,
+                                             const int32_t* text_len_dev, float* mass, void* workspace, int64_t workspace_bytes, void* out,
+                                             int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t n_pages, int32_t table_width,
+                                             int32_t page_size, int32_t window, int32_t sinks, float scale) {
+  const char* op = "vle_op_paged_decode_attention";
+  if (const char* e = heads_fault(dtype, nhead, nhead_kv, dh)) return op_refuse(op, e);
+  if (const char* e = cache_fault(B, nhead_kv, dh, n_pages, table_width, page_size)) return op_refuse(op, e);
+  if (window < 0 || sinks < 0) return op_refuse(op, "window and sinks must not be negative");
+  if (!(scale > 0.f) || scale > 3.0e38f) return op_refuse(op, "scale must be positive and finite");
+  if (B == 0) return VLE_OK;
+  if (!q || !k_pages || !v_pages || !page_table_dev || !lengths_dev || !out) return op_refuse(op, "null operand");
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || !vec_strides(dtype, q_row, q_head))
+    return op_refuse(op, "rows and heads must start on 16 bytes");
+  const PagedDecodePlan p = paged_decode_plan(B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, text_len_dev != nullptr, mass != nullptr);
+  const int64_t need = (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return op_refuse(op, "workspace too small (vle_op_paged_decode_workspace_bytes)");
+  PagedDecodeArgs a;
+  a.q = q; a.q_b = q_row; a.q_h = q_head; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.mass = mass;
+  a.table = page_table_dev; a.lengths = lengths_dev; a.text_len = text_len_dev;
+  float* ws = (float*)workspace;
+  a.scores = p.score_floats ? ws : nullptr;
+  a.part_o = p.o_floats ? ws + p.score_floats : nullptr;
+  a.part_ml = p.ml_floats ? ws + p.score_floats + p.o_floats : nullptr;
+  a.Hkv = nhead_kv; a.G = nhead / nhead_kv; a.dh = dh; a.n_pages = n_pages; a.W = table_width; a.psl = log2_of(page_size);
+  a.window = window; a.sinks = sinks; a.sl2 = scale * 1.4426950408889634f;
+  return op_done(launch_paged_decode((hipStream_t)stream, dtype, p, a, B), op);
+}
+
+extern "C" int vle_op_kv_evict(void* stream, int dtype, void* k_pages, void* v_pages, float* mass, const int32_t* page_table_dev,
+                               const int32_t* lengths_dev, const int32_t* text_len_dev, int32_t* kept, int32_t* new_lengths, int32_t B,
+                               int32_t nhead_kv, int32_t dh, int32_t n_pages, int32_t table_width, int32_t page_size, int32_t budget,
+                               int32_t recent, int32_t sinks) {
+  const char* op = "vle_op_kv_evict";
+  if (const char* e = heads_fault(dtype, nhead_kv, nhead_kv, dh)) return op_refuse(op, e);
+  if (const char* e = cache_fault(B, nhead_kv, dh, n_pages, table_width, page_size)) return op_refuse(op, e);
+  if (budget < 1 || budget > (1 << 25)) return op_refuse(op, "budget must be 1 to 2^25");
+  if (recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget) return op_refuse(op, "sinks and recent keys must fit the budget");
+  if (B == 0) return VLE_OK;
+  if (!k_pages || !v_pages || !mass || !page_table_dev || !lengths_dev || !kept || !new_lengths) return op_refuse(op, "null operand");
+  if (k_pages == v_pages) return op_refuse(op, "keys and values need pages of their own");
+  if (!aligned16(k_pages) || !aligned16(v_pages)) return op_refuse(op, "pages must start on 16 bytes");
+  EvictArgs a;
+  a.k_pages = k_pages; a.v_pages = v_pages; a.mass = mass; a.table = page_table_dev; a.lengths = lengths_dev; a.text_len = text_len_dev;
+  a.kept = kept; a.new_lengths = new_lengths; a.Hkv = nhead_kv; a.n_pages = n_pages; a.W = table_width; a.psl = log2_of(page_size);
+  a.budget = budget; a.recent = recent; a.sinks = sinks;
+  return op_done(launch_kv_evict((hipStream_t)stream, dtype, a, B, dh), op);
 }

@@ -1,0 +1,549 @@
+// Prompt attention with a sliding window, first tokens that stay visible (sinks), a text prefix that every row sees, and grouped heads.
+//
+//   out_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale q_i . k_j
+//   row i of a sequence sees key j  iff  j < text  or  (j <= i and (window <= 0 or i - j < window or j < sinks))
+//
+// One workgroup takes a run of query rows of one (sequence, head) and walks the key tiles that any of them sees: the tiles of the head
+// (text, sinks), then those of the window; the tiles between are never loaded, so the work of a row is its window's, not its position's.
+// Both products are computed transposed (S^T = K Q^T, O^T = V^T P^T): the weights leave the first in the operand layout of the second.
+// The scores' running maximum, the row sums and both accumulators are fp32.  A lane holds the query column c = lane % 16 and of every 16-key
+// score tile the keys 4 g + r, g = lane / 16.
+//
+// A key that a row does not see must not reach it, whatever it holds -- but a tile's product runs over all keys of the tile, and 0 * NaN is NaN.
+// Rows whose result is not finite (a rarity: such a value, or sums past the largest number) are therefore computed once more, key by key over
+// the visible ones alone (exact_row).
+#include "common.h"
+#include "kernels.h"
+
+namespace vle {
+
+namespace {
+
+typedef __bf16 wa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 wa_bf16x4 __attribute__((ext_vector_type(4)));
+typedef short wa_s16x4 __attribute__((ext_vector_type(4)));
+typedef short wa_s16x8 __attribute__((ext_vector_type(8)));
+typedef float wa_f32x4 __attribute__((ext_vector_type(4)));
+typedef float wa_f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned wa_u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float WA_DEFER = 8.f;  // exp2-domain growth of a row's maximum below which its reference stays (weights up to 2^8)
+
+// Where a workgroup works: sequence, head, first query row.  Work items are numbered head by head, a sequence's row runs one after another
+// (late ones, which see most without a window, first), so that neighbours read the same keys; `seq` = -1: no sequence is left for this item and
+// `rest` counts the items past the last one.
+struct Place {
+  int h, seq, off, len, q0, rest;
+};
+template <int QB>
+__device__ inline Place place_of(const WindowAttnArgs& a) {
+  const int lane = threadIdx.x & 63;
+  const int per_head = gridDim.x / a.H;
+  // workgroup L runs on XCD L % 8, each with its own L2: every XCD gets a contiguous run of the items
+  const int nb = gridDim.x, q = nb / 8, rem = nb % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
+  const int item = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + idx;
+  Place p;
+  p.h = item / per_head;
+  int at = item - p.h * per_head;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    int off = 0, len = 0;
+    if (b < a.B) {
+      off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
+      len = (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
+    }
+    const int runs = (len + QB - 1) / QB;
+    int inc = runs;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += t;
+    }
+    const unsigned long long past = __ballot(at < inc);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      p.seq = b0 + l;
+      p.off = __builtin_amdgcn_readlane(off, l);
+      p.len = __builtin_amdgcn_readlane(len, l);
+      p.q0 = (__builtin_amdgcn_readlane(inc, l) - 1 - at) * QB;
+      p.rest = 0;
+      return p;
+    }
+    at -= __builtin_amdgcn_readlane(inc, 63);
+  }
+  p.seq = -1;
+  p.off = p.len = p.q0 = 0;
+  p.rest = at;
+  return p;
+}
+
+// The key tiles a run of rows i0 .. i1 sees (TK keys each): 0 .. th - 1 the head, then mf + (t - th).
+struct Tiles {
+  int th, mf, tt;
+};
+template <int TK>
+__device__ inline Tiles tiles_of(int i0, int i1, int text, int window, int sinks) {
+  Tiles r;
+  const int hd = window > 0 ? max(text, min(sinks, i1 + 1)) : text;
+  const int lo = window > 0 ? max(0, i0 - window + 1) : 0;
+  r.th = (hd + TK - 1) / TK;
+  r.mf = max(r.th, lo / TK);
+  r.tt = r.th + max(0, (i1 + TK) / TK - r.mf);
+  return r;
+}
+
+// What one row sees: keys j < hd, and lo <= j <= i.
+struct Sight {
+  int hd, lo, i;
+  __device__ bool sees(int j) const { return j < hd || (j >= lo && j <= i); }
+  __device__ bool all(int j0, int n) const { return j0 + n <= hd || (j0 >= lo && j0 + n - 1 <= i); }
+  __device__ bool any(int j0, int n) const { return j0 < hd || (j0 <= i && j0 + n - 1 >= lo); }
+};
+__device__ inline Sight sight_of(int i, int text, int window, int sinks) {
+  Sight s;
+  s.hd = window > 0 ? max(text, min(sinks, i + 1)) : text;
+  s.lo = window > 0 ? max(0, i - window + 1) : 0;
+  s.i = i;
+  return s;
+}
+
+__device__ inline float wa_elem(const void* p, int64_t i, bool bf) { return bf ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i]; }
+
+// One row over its visible keys alone, by one wave: 64 keys at a time, a lane the score of one, then two elements of the output.
+template <typename T>
+__device__ inline void exact_row(const WindowAttnArgs& a, int h, int off, int i, int text, int len) {
+#pragma clang fp contract(off)  // score - m must be the difference of two rounded scores: 0 for the largest, whatever its size
+  constexpr bool BF = sizeof(T) == 2;
+  const int lane = threadIdx.x & 63, hk = h / (a.H / a.Hkv);
+  const Sight see = sight_of(i, text, a.window, a.sinks);
+  const int64_t qo = (int64_t)(off + i) * a.q_row + (int64_t)h * a.q_head;
+  auto score = [&](int j) -> float {
+    const int64_t ko = (int64_t)(off + j) * a.k_row + (int64_t)hk * a.k_head;
+    float s = 0.f;
+    for (int e = 0; e < a.dh; ++e) s = fmaf(wa_elem(a.q, qo + e, BF), wa_elem(a.k, ko + e, BF), s);
+    return s * a.sl2;
+  };
+  const int end = min(len, max(see.hd, i + 1));
+  float m = -INFINITY;
+  bool nan = false;
+  for (int j = lane; j < end; j += 64)
+    if (see.sees(j)) {
+      const float s = score(j);
+      nan |= s != s;
+      m = fmaxf(m, s);
+    }
+  m = wave_max(m);
+  if (__any(nan)) m = __builtin_nanf("");
+  float l = 0.f;
+  for (int j = lane; j < end; j += 64)
+    if (see.sees(j)) l += __builtin_amdgcn_exp2f(score(j) - m);
+  l = wave_sum(l);
+  float o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 < end; j0 += 64) {
+    const int j = j0 + lane;
+    const bool vis = j < end && see.sees(j);
+    const float p = vis ? __builtin_amdgcn_exp2f(score(j) - m) / l : 0.f;
+    unsigned long long todo = __ballot(vis);
+    while (todo) {
+      const int t = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const float w = readlane_f32(p, t);
+      const int64_t vo = (int64_t)(off + j0 + t) * a.v_row + (int64_t)hk * a.v_head;
+      if (lane < a.dh) o0 = fmaf(w, wa_elem(a.v, vo + lane, BF), o0);
+      if (lane + 64 < a.dh) o1 = fmaf(w, wa_elem(a.v, vo + lane + 64, BF), o1);
+    }
+  }
+  T* op = (T*)a.out + ((int64_t)(off + i) * a.H + h) * a.dh;
+  if (lane < a.dh) store_elem<T>(op + lane, o0);
+  if (lane + 64 < a.dh) store_elem<T>(op + lane + 64, o1);
+}
+
+// Rows that no sequence holds, `rest`-th run of them.
+template <typename T, int QB>
+__device__ inline void zero_rows(const WindowAttnArgs& a, int h, int rest) {
+  const int first = a.B > 0 ? (int)min((int64_t)max(a.seq_off[0], 0), a.rows) : 0;
+  const int64_t end = a.B > 0 ? min((int64_t)max(a.seq_off[a.B], first), a.rows) : 0;
+  const int vpr = a.dh * (int)sizeof(T) / 16;
+  for (int idx = threadIdx.x; idx < QB * vpr; idx += blockDim.x) {
+    int64_t r = (int64_t)rest * QB + idx / vpr;
+    if (r >= first) r += end - first;
+    if (r >= a.rows) return;
+    reinterpret_cast<wa_u32x4*>((T*)a.out + (r * a.H + h) * a.dh)[idx % vpr] = wa_u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// 16-byte slot swizzle of the LDS rows (NV slots each), applied to the address a DMA lane fetches from and to every read: rows land on
+// different banks.  The key stays inside an aligned group of slots that divides NV.
+template <int NV>
+__device__ constexpr int wa_key(int row) {
+  return NV % 16 == 0 ? (row & 15) : NV % 8 == 0 ? (row & 7) : ((row >> 1) & 3);
+}
+
+__device__ inline void wa_dma(const void* src, unsigned char* dst) {  // 16 bytes per lane to dst + 16 * lane (dst wave-uniform)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// One tile of TK rows (NV vectors of VE elements each) of K or V into LDS, by the whole workgroup.  Rows past the sequence repeat its last one
+// and vectors past the head its first one: what they hold is never visible.
+template <typename T, int TK, int NV>
+__device__ inline void stage_tile(const T* base, int64_t row_stride, int kt0, int len, int dh, unsigned char* dst, int w_uniform) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < TK * NV / 256; ++i) {
+    const int idx = (i * 4 + w) * 64 + lane;
+    const int row = idx / NV, slot = idx % NV;
+    int vec = slot ^ wa_key<NV>(row);
+    if (vec * VE >= dh) vec = 0;
+    wa_dma(base + (int64_t)min(kt0 + row, len - 1) * row_stride + vec * VE, dst + (i * 4 + w_uniform) * 1024);
+  }
+}
+
+}  // namespace
+
+// ---- bf16 --------------------------------------------------------------------------------------------------------------------------
+// 4 waves, QW query fragments of 16 rows each; 64-key tiles of K and V go global -> LDS by DMA into one of two buffers while the other is
+// multiplied; V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the matrix pipe (an all-ones
+// row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16 (8 bits: 2^-9 of each weight, which
+// averages out over the keys and stays below the output's own rounding).
+template <int DHT, int QW>
+__global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a) {
+  constexpr int QB = 64 * QW, TK = 64, NV = DHT / 8, ROW = DHT * 2, KS = DHT / 32, EB = DHT / 16;
+  constexpr int HALF = TK * ROW, BUF = 2 * HALF;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BUF];
+  const Place pl = place_of<QB>(a);
+  if (pl.seq < 0) {
+    if (a.zero_rest) zero_rows<bf16_t, QB>(a, pl.h, pl.rest);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  const int len = pl.len, q0 = pl.q0, dh = a.dh, hk = pl.h / (a.H / a.Hkv);
+  const int text = a.text_len ? min(max(a.text_len[pl.seq], 0), len) : 0;
+  const Tiles ti = tiles_of<TK>(q0, min(q0 + QB, len) - 1, text, a.window, a.sinks);
+  const bf16_t* kb = (const bf16_t*)a.k + (int64_t)pl.off * a.k_row + (int64_t)hk * a.k_head;
+  const bf16_t* vb = (const bf16_t*)a.v + (int64_t)pl.off * a.v_row + (int64_t)hk * a.v_head;
+
+  Sight see[QW];
+  bool valid[QW];
+  wa_bf16x8 qf[QW][KS];
+#pragma unroll
+  for (int f = 0; f < QW; ++f) {
+    const int i = q0 + (w * QW + f) * 16 + c;
+    valid[f] = i < len;
+    see[f] = sight_of(min(i, len - 1), text, a.window, a.sinks);
+    const bf16_t* qp = (const bf16_t*)a.q + (int64_t)(pl.off + min(i, len - 1)) * a.q_row + (int64_t)pl.h * a.q_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      wa_u32x4 x = {0u, 0u, 0u, 0u};
+      if (ks * 32 + g * 8 < dh) x = *reinterpret_cast<const wa_u32x4*>(qp + ks * 32 + g * 8);
+      qf[f][ks] = __builtin_bit_cast(wa_bf16x8, x);
+    }
+  }
+
+  const float sl2 = a.sl2, defer = WA_DEFER / a.sl2;
+  float m[QW];  // running maximum of the raw scores of the row, shared by its 4 lanes
+  wa_f32x4 ol[QW], o[QW][EB];
+#pragma unroll
+  for (int f = 0; f < QW; ++f) {
+    m[f] = -INFINITY;
+    ol[f] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int eb = 0; eb < EB; ++eb) o[f][eb] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const wa_bf16x8 ones = __builtin_bit_cast(wa_bf16x8, wa_s16x8{0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80});
+  auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
+
+  stage_tile<bf16_t, TK, NV>(kb, a.k_row, key0(0), len, dh, smem, wu);
+  stage_tile<bf16_t, TK, NV>(vb, a.v_row, key0(0), len, dh, smem + HALF, wu);
+  for (int t = 0; t < ti.tt; ++t) {
+    const int kt0 = key0(t);
+    const unsigned char* Ks = smem + (t & 1) * BUF;
+    const unsigned char* Vs = Ks + HALF;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's pieces of tile t have landed
+    __syncthreads();                                  // everyone's have; everyone is done with tile t - 1
+    if (t + 1 < ti.tt) {
+      unsigned char* nb = smem + ((t + 1) & 1) * BUF;
+      stage_tile<bf16_t, TK, NV>(kb, a.k_row, key0(t + 1), len, dh, nb, wu);
+      stage_tile<bf16_t, TK, NV>(vb, a.v_row, key0(t + 1), len, dh, nb + HALF, wu);
+    }
+    bool some = false, all = true;
+#pragma unroll
+    for (int f = 0; f < QW; ++f) {
+      some |= see[f].any(kt0, TK);
+      all &= see[f].all(kt0, TK);
+    }
+    if (!__any(some)) continue;
+    const bool unmasked = __all(all);
+
+    // ---- S^T = K Q^T ----
+    wa_f32x4 s[QW][4];
+#pragma unroll
+    for (int kb4 = 0; kb4 < 4; ++kb4) {
+#pragma unroll
+      for (int f = 0; f < QW; ++f) s[f][kb4] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const wa_bf16x8 ka = *reinterpret_cast<const wa_bf16x8*>(Ks + (kb4 * 16 + c) * ROW + (((ks * 4 + g) ^ wa_key<NV>(c)) << 4));
+#pragma unroll
+        for (int f = 0; f < QW; ++f) s[f][kb4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[f][ks], s[f][kb4], 0, 0, 0);
+      }
+    }
+    // ---- online softmax ----
+    wa_bf16x8 pf[QW][2];
+#pragma unroll
+    for (int f = 0; f < QW; ++f) {
+      if (!unmasked) {
+#pragma unroll
+        for (int kb4 = 0; kb4 < 4; ++kb4)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!see[f].sees(kt0 + kb4 * 16 + g * 4 + r)) s[f][kb4][r] = -INFINITY;
+      }
+      float mt = fmaxf(fmaxf(s[f][0][0], s[f][0][1]), fmaxf(s[f][0][2], s[f][0][3]));
+#pragma unroll
+      for (int kb4 = 1; kb4 < 4; ++kb4) mt = fmaxf(mt, fmaxf(fmaxf(s[f][kb4][0], s[f][kb4][1]), fmaxf(s[f][kb4][2], s[f][kb4][3])));
+      // the reference stays while no score exceeds it by more than `defer`: the result does not depend on it, O and the sum carry the same factor
+      if (!__all(mt <= m[f] + defer)) {
+        const float mn = fmaxf(m[f], rows4_max(mt));
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f((m[f] - ref) * sl2);
+        m[f] = mn;
+        ol[f] *= alpha;
+#pragma unroll
+        for (int eb = 0; eb < EB; ++eb) o[f][eb] *= alpha;
+      }
+      // s sl2 - m sl2 in one fma: what the rounding of m sl2 leaves is a factor of the whole row and cancels, up to scores of 2^31, where it
+      // passes the exponent's range and the row is computed again
+      const float nm = m[f] == -INFINITY ? 0.f : -m[f] * sl2;
+#pragma unroll
+      for (int kb4 = 0; kb4 < 4; ++kb4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[f][kb4][r] = __builtin_amdgcn_exp2f(fmaf(s[f][kb4][r], sl2, nm));
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int tt = 0; tt < 8; ++tt) pf[f][j][tt] = (__bf16)s[f][2 * j + (tt >> 2)][tt & 3];
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int f = 0; f < QW; ++f) ol[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[f][j], ol[f], 0, 0, 0);
+#pragma unroll
+    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // the transposing read hands lane c the elements V[k0 .. k0 + 3][16 eb + c] of the rows whose addresses lanes c / 4 supply
+        const int key = j * 32 + g * 4 + (c >> 2);
+        const unsigned char* va = Vs + key * ROW + (((eb * 2 + ((c & 3) >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3);
+        const unsigned char* vh = va + 16 * ROW;  // the key of the swizzle has a period of 16 rows
+        const wa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va));
+        const wa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(vh));
+        const wa_bf16x8 vf = __builtin_bit_cast(wa_bf16x8, wa_s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+#pragma unroll
+        for (int f = 0; f < QW; ++f) o[f][eb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][j], o[f][eb], 0, 0, 0);
+      }
+  }
+
+#pragma unroll
+  for (int f = 0; f < QW; ++f) {
+    const float inv = 1.0f / ol[f][0];  // every row of the all-ones block holds the whole sum
+    const int i = q0 + (w * QW + f) * 16 + c;
+    bool odd = false;
+    bf16_t* op = (bf16_t*)a.out + ((int64_t)(pl.off + i) * a.H + pl.h) * dh + g * 4;
+#pragma unroll
+    for (int eb = 0; eb < EB; ++eb) {
+      if (eb * 16 + g * 4 >= dh) continue;
+      wa_bf16x4 r4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = o[f][eb][r] * inv;
+        odd |= !(fabsf(x) < INFINITY);
+        r4[r] = (__bf16)x;
+      }
+      if (valid[f]) *reinterpret_cast<wa_bf16x4*>(op + eb * 16) = r4;
+    }
+    unsigned long long again = __ballot(odd && valid[f]);
+    if (again) {
+      again = (again | (again >> 16) | (again >> 32) | (again >> 48)) & 0xffffull;
+      while (again) {
+        const int t = __builtin_ctzll(again);
+        again &= again - 1;
+        exact_row<bf16_t>(a, pl.h, pl.off, q0 + (wu * QW + f) * 16 + t, text, len);
+      }
+    }
+  }
+}
+
+// ---- fp32 --------------------------------------------------------------------------------------------------------------------------
+// The same walk on v_mfma_f32_16x16x4_f32 (exact fp32 products, 1/16 of the bf16 rate): 64 query rows, 32-key tiles.  A 16-byte fragment of
+// K feeds four products (contraction slot g of product u is dim 16 t + 4 g + u); V^T needs no transpose: product j of key r takes V[4 g + r][dim(c, j)],
+// with dim(c, j) the j-th of the up to 8 elements that lane c reads of a row.
+template <int DHT>
+__global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) {
+  constexpr int QB = 64, TK = 32, NV = DHT / 4, ROW = DHT * 4, KT = DHT / 16, DPL = DHT / 16;
+  constexpr int HALF = TK * ROW, BUF = 2 * HALF;
+  constexpr int A4 = DPL >= 4 ? 4 : 2;           // elements of a lane's first chunk of a V row, and of its second
+  constexpr int B4 = DPL - A4;                   // (DHT 32: 2, 64: 4, 96: 4 + 2, 128: 4 + 4)
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BUF];
+  const Place pl = place_of<QB>(a);
+  if (pl.seq < 0) {
+    if (a.zero_rest) zero_rows<float, QB>(a, pl.h, pl.rest);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  const int len = pl.len, q0 = pl.q0, dh = a.dh, hk = pl.h / (a.H / a.Hkv);
+  const int text = a.text_len ? min(max(a.text_len[pl.seq], 0), len) : 0;
+  const Tiles ti = tiles_of<TK>(q0, min(q0 + QB, len) - 1, text, a.window, a.sinks);
+  const float* kb = (const float*)a.k + (int64_t)pl.off * a.k_row + (int64_t)hk * a.k_head;
+  const float* vb = (const float*)a.v + (int64_t)pl.off * a.v_row + (int64_t)hk * a.v_head;
+  const int i = q0 + w * 16 + c;
+  const bool valid = i < len;
+  const Sight see = sight_of(min(i, len - 1), text, a.window, a.sinks);
+  wa_f32x4 qf[KT];
+  const float* qp = (const float*)a.q + (int64_t)(pl.off + min(i, len - 1)) * a.q_row + (int64_t)pl.h * a.q_head;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    qf[t] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+    if (t * 16 + g * 4 < dh) qf[t] = *reinterpret_cast<const wa_f32x4*>(qp + t * 16 + g * 4);
+  }
+  const float sl2 = a.sl2;
+  float m = -INFINITY, l = 0.f;
+  wa_f32x4 o[DPL];
+#pragma unroll
+  for (int j = 0; j < DPL; ++j) o[j] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+  auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
+
+  stage_tile<float, TK, NV>(kb, a.k_row, key0(0), len, dh, smem, wu);
+  stage_tile<float, TK, NV>(vb, a.v_row, key0(0), len, dh, smem + HALF, wu);
+  for (int t = 0; t < ti.tt; ++t) {
+    const int kt0 = key0(t);
+    const unsigned char* Ks = smem + (t & 1) * BUF;
+    const unsigned char* Vs = Ks + HALF;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t + 1 < ti.tt) {
+      unsigned char* nb = smem + ((t + 1) & 1) * BUF;
+      stage_tile<float, TK, NV>(kb, a.k_row, key0(t + 1), len, dh, nb, wu);
+      stage_tile<float, TK, NV>(vb, a.v_row, key0(t + 1), len, dh, nb + HALF, wu);
+    }
+    if (!__any(see.any(kt0, TK))) continue;
+    wa_f32x4 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t4 = 0; t4 < KT; ++t4) {
+        const wa_f32x4 ka = *reinterpret_cast<const wa_f32x4*>(Ks + (kt * 16 + c) * ROW + (((t4 * 4 + g) ^ wa_key<NV>(c)) << 4));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[u], qf[t4][u], s[kt], 0, 0, 0);
+      }
+    }
+    const bool unmasked = __all(see.all(kt0, TK));
+    float mt = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (!unmasked && !see.sees(kt0 + kt * 16 + g * 4 + r)) s[kt][r] = -INFINITY;
+        mt = fmaxf(mt, s[kt][r]);
+      }
+    mt = rows4_max(mt);
+    const float mn = fmaxf(m, mt);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f((m - ref) * sl2);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[kt][r] = __builtin_amdgcn_exp2f((s[kt][r] - ref) * sl2);
+        sum += s[kt][r];
+      }
+    l = fmaf(l, alpha, sum);
+    if (!__all(alpha == 1.0f)) {
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) o[j] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = kt * 16 + g * 4 + r;
+        const unsigned char* row = Vs + key * ROW;
+        float vv[DPL];
+        if constexpr (A4 == 4) {
+          const wa_f32x4 x = *reinterpret_cast<const wa_f32x4*>(row + ((c ^ wa_key<NV>(key)) << 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vv[j] = x[j];
+          if constexpr (B4 == 4) {
+            const wa_f32x4 y = *reinterpret_cast<const wa_f32x4*>(row + (((16 + c) ^ wa_key<NV>(key)) << 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vv[4 + j] = y[j];
+          } else if constexpr (B4 == 2) {
+            const wa_f32x2 y = *reinterpret_cast<const wa_f32x2*>(row + (((16 + (c >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
+            vv[4] = y[0];
+            vv[5] = y[1];
+          }
+        } else {
+          const wa_f32x2 x = *reinterpret_cast<const wa_f32x2*>(row + (((c >> 1) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
+          vv[0] = x[0];
+          vv[1] = x[1];
+        }
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[j], s[kt][r], o[j], 0, 0, 0);
+      }
+  }
+  l = rows4_sum(l);
+  bool odd = false;
+  float* op = (float*)a.out + ((int64_t)(pl.off + i) * a.H + pl.h) * dh;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int slot = 4 * g + r;
+#pragma unroll
+    for (int j = 0; j < DPL; j += 2) {
+      const int e = j < A4 ? A4 * slot + j : 16 * A4 + B4 * slot + (j - A4);
+      if (e >= dh) continue;
+      const wa_f32x2 x = {o[j][r] / l, o[j + 1][r] / l};
+      odd |= !(fabsf(x[0]) < INFINITY) || !(fabsf(x[1]) < INFINITY);
+      if (valid) *reinterpret_cast<wa_f32x2*>(op + e) = x;
+    }
+  }
+  unsigned long long again = __ballot(odd && valid);
+  if (again) {
+    again = (again | (again >> 16) | (again >> 32) | (again >> 48)) & 0xffffull;
+    while (again) {
+      const int t = __builtin_ctzll(again);
+      again &= again - 1;
+      exact_row<float>(a, pl.h, pl.off, q0 + wu * 16 + t, text, len);
+    }
+  }
+}
+
+int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) {
+  if (a.rows <= 0) return 0;
+  const bool f32 = dtype == DT_F32;
+  // items of a head: the rows' runs, one more for every sequence's ragged last one, one for the rows of no sequence
+  auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
+  const bool wide = !f32 && items(128) * a.H >= 1024;
+  const int64_t n = items(wide ? 128 : 64) * a.H;
+  if (n > 0x7fffffff) return -1;
+  const dim3 grid((unsigned)n), block(256);
+#define VLE_WA(DHT)                                                                             \
+  do {                                                                                          \
+    if (f32) hipLaunchKernelGGL((window_attn_f32_kernel<DHT>), grid, block, 0, st, a);          \
+    else if (wide) hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 2>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 1>), grid, block, 0, st, a);          \
+  } while (0)
+  if (a.dh <= 32) VLE_WA(32);
+  else if (a.dh <= 64) VLE_WA(64);
+  else if (a.dh <= 96) VLE_WA(96);
+  else VLE_WA(128);
+#undef VLE_WA
+  return 0;
+}
+
+}  // namespace vle
