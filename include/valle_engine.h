@@ -405,7 +405,7 @@ int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int64_t k_row,
                           int64_t v_head, void* k_pages, void* v_pages, float* mass, const int32_t* page_table_dev,
                           const int32_t* start_dev, const int32_t* seq_off_dev, int64_t rows, int32_t B, int32_t nhead_kv, int32_t dh,
                           int32_t n_pages, int32_t table_width, int32_t page_size);
-int64_t vle_op_paged_decode_workspace_bytes(int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
+int64_t vle_op_paged_decode_workspace_bytes(int dtype, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
                                             int32_t page_size, int32_t window, int32_t sinks, int32_t has_text, int32_t has_mass);
 int vle_op_paged_decode_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
                                   const void* v_pages, const int32_t* page_table_dev, const int32_t* lengths_dev,

@@ -116,7 +116,7 @@ def _c_decode(dtype=0, k=P, B=2, H=4, Hkv=2, dh=16, n_pages=3, W=2, ps=8, window
 
 @pytest.mark.parametrize("kw", [dict(dtype=2), dict(H=5), dict(dh=20), dict(n_pages=0), dict(W=0), dict(ps=4), dict(ps=24), dict(W=2**20, ps=1024),
                                 dict(B=70000), dict(window=-1), dict(sinks=-2), dict(scale=0.0), dict(k=None), dict(k=C.c_void_p(4104)),
-                                dict(mass=P), dict(mass=P, ws=P, ws_bytes=16), dict(W=4096, B=1), dict(Hkv=2, H=2, ps=2**24, W=1)])
+                                dict(mass=P, W=2000), dict(mass=P, W=2000, ws=P, ws_bytes=16), dict(W=4096, B=1), dict(Hkv=2, H=2, ps=2**24, W=1)])
 def test_c_paged_decode_refuses(kw):
     assert _c_decode(**kw) == _lib.VLE_EINVAL
     assert b"vle_op_paged_decode_attention" in _lib.load().vle_last_error(None)
@@ -124,14 +124,14 @@ def test_c_paged_decode_refuses(kw):
 
 def test_c_workspace_query():
     lib = _lib.load()
-    assert lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 64, 8, 16, 0, 0, 0, 0) == 0  # short: one launch, no workspace
-    short = lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 64, 8, 16, 0, 0, 0, 1)
-    assert short >= 16 * 8 * 16 * 4  # every score
-    assert lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 64, 8192, 16, 0, 0, 0, 0) > 0
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8, 16, 0, 0, 0, 0) == 0  # short: one launch, no workspace
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8, 16, 0, 0, 0, 1) == 0  # its scores fit the LDS
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 1, 64, 64, 16, 0, 0, 0, 1) >= 16 * 1024 * 4  # every score
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8192, 16, 0, 0, 0, 0) > 0
     # a window bounds the scores kept, whatever the table's width; a text of unknown length does not
-    wide, bounded = (lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 64, 8192, 16, w, 4, 0, 1) for w in (0, 500))
-    assert bounded < wide // 50 and lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 64, 8192, 16, 500, 4, 1, 1) > wide // 2
-    assert lib.vle_op_paged_decode_workspace_bytes(1, 16, 16, 60, 8, 16, 0, 0, 0, 0) == _lib.VLE_EINVAL
+    wide, bounded = (lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8192, 16, w, 4, 0, 1) for w in (0, 500))
+    assert bounded < wide // 50 and lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8192, 16, 500, 4, 1, 1) > wide // 2
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 60, 8, 16, 0, 0, 0, 0) == _lib.VLE_EINVAL
 
 
 def _c_write(dtype=0, rows=2, B=2, Hkv=2, dh=16, n_pages=3, W=2, ps=8, off=None, k=P, row=32):

@@ -85,7 +85,7 @@ SIGNATURES = {
                                           C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float, C.c_int32]),
     "vle_op_paged_kv_write": (C.c_int, [_P, C.c_int, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64,
                                         C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
-    "vle_op_paged_decode_workspace_bytes": (C.c_int64, [C.c_int32] * 10),
+    "vle_op_paged_decode_workspace_bytes": (C.c_int64, [C.c_int] + [C.c_int32] * 10),
     "vle_op_paged_decode_attention": (C.c_int, [_P, C.c_int, _P, C.c_int64, C.c_int64, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P] + [C.c_int32] * 9
                                       + [C.c_float]),
     "vle_op_kv_evict": (C.c_int, [_P, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P] + [C.c_int32] * 9),

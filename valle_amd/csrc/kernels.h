@@ -515,14 +515,14 @@ struct PagedDecodeArgs {
   int Hkv, G, dh, n_pages, W, psl, window, sinks;
   float sl2;
   // set by the launcher
-  int GT, chunk, nsplit;
+  int GT, nsplit, score_lds, join_heads;
   int64_t score_ld;
 };
 struct PagedDecodePlan {  // split of the cache's length, and the workspace it needs
-  int tiles, chunk, nsplit, nw;
+  int tiles, nsplit, nw, score_lds;  // score_lds > 0: scores of a head kept in LDS
   size_t ml_floats, o_floats, score_floats;
 };
-PagedDecodePlan paged_decode_plan(int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass);
+PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass);
 int launch_paged_decode(hipStream_t st, int dtype, const PagedDecodePlan& p, PagedDecodeArgs a, int B);
 
 struct EvictArgs {

@@ -356,14 +356,14 @@ extern "C" int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int
   return op_done(launch_paged_write((hipStream_t)stream, dtype, a), op);
 }
 
-extern "C" int64_t vle_op_paged_decode_workspace_bytes(int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
+extern "C" int64_t vle_op_paged_decode_workspace_bytes(int dtype, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh, int32_t table_width,
                                                        int32_t page_size, int32_t window, int32_t sinks, int32_t has_text, int32_t has_mass) {
   const char* op = "vle_op_paged_decode_workspace_bytes";
-  const char* e = heads_fault(DT_F32, nhead, nhead_kv, dh);
+  const char* e = heads_fault(dtype, nhead, nhead_kv, dh);
   if (!e) e = cache_fault(B, nhead_kv, dh, 1, table_width, page_size);
   if (!e && (window < 0 || sinks < 0)) e = "window and sinks must not be negative";
   if (e) return op_refuse(op, e);
-  const PagedDecodePlan p = paged_decode_plan(B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, has_text != 0, has_mass != 0);
+  const PagedDecodePlan p = paged_decode_plan(dtype, B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, has_text != 0, has_mass != 0);
   return (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
 }
 
@@ -381,7 +381,7 @@ extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void
   if (!q || !k_pages || !v_pages || !page_table_dev || !lengths_dev || !out) return op_refuse(op, "null operand");
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || !vec_strides(dtype, q_row, q_head))
     return op_refuse(op, "rows and heads must start on 16 bytes");
-  const PagedDecodePlan p = paged_decode_plan(B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, text_len_dev != nullptr, mass != nullptr);
+  const PagedDecodePlan p = paged_decode_plan(dtype, B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, text_len_dev != nullptr, mass != nullptr);
   const int64_t need = (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need)) return op_refuse(op, "workspace too small (vle_op_paged_decode_workspace_bytes)");
   PagedDecodeArgs a;

@@ -20,35 +20,40 @@ typedef float pc_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned pc_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned pc_u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int PC_TILE = 32;  // keys of one wave step: two 16-key score tiles feed one K = 32 MFMA of the weights
+// Keys of one wave step: bf16 32 (two 16-key score tiles feed one product with 32 contraction slots), fp32 16 (64 registers for its keys and values).
+template <typename T>
+constexpr int pc_tile() { return sizeof(T) == 4 ? 16 : 32; }
 
-// The keys the newest token of a sequence sees: j < n and (j < hd or j >= lo), as tiles of 32 keys.  Tiles 0 .. th - 1 cover the head,
-// tile t >= th starts at key (mf + t - th) * 32; tiles between the head and the window are never touched.
+// The keys the newest token of a sequence sees: j < n and (j < hd or j >= lo), as tiles of TK keys.  Tiles 0 .. th - 1 cover the head,
+// tile t >= th starts at key (mf + t - th) * TK; tiles between the head and the window are never touched.
+template <int TK>
 struct Span {
   int n, hd, lo, th, mf, tt;
-  __device__ int key0(int t) const { return (t < th ? t : mf + (t - th)) * PC_TILE; }
-  __device__ bool sees(int j) const { return j < n && (j < hd || j >= lo); }
+  __device__ int key0(int t) const { return (t < th ? t : mf + (t - th)) * TK; }
+  // (& and | on purpose: a select per key, no branches)
+  __device__ bool sees(int j) const { return (j < n) & ((j < hd) | (j >= lo)); }
+  __device__ bool sees_tile(int j0) const { return (j0 + TK <= n) & ((j0 + TK <= hd) | (j0 >= lo)); }
 };
 
-__device__ inline Span span_of(int n, int text, int window, int sinks) {
-  Span s;
-  s.n = n;
-  if (window <= 0 || window >= n) {
-    s.hd = s.lo = n;
+template <int TK>
+__device__ inline Span<TK> span_of_row(const PagedDecodeArgs& a, int b) {
+  Span<TK> s;
+  s.n = min(max(a.lengths[b], 0), a.W << a.psl);  // W * ps < 2^30 (checked at the entry)
+  if (a.window <= 0 || a.window >= s.n) {
+    s.hd = s.lo = s.n;
   } else {
-    s.hd = min(n, max(text, sinks));
-    s.lo = n - window;
+    s.hd = min(s.n, max(a.text_len ? a.text_len[b] : 0, a.sinks));
+    s.lo = s.n - a.window;
   }
-  s.th = (s.hd + PC_TILE - 1) / PC_TILE;
-  s.mf = max(s.th, s.lo / PC_TILE);
-  s.tt = s.th + max(0, (n + PC_TILE - 1) / PC_TILE - s.mf);
+  s.th = (s.hd + TK - 1) / TK;
+  s.mf = max(s.th, s.lo / TK);
+  s.tt = s.th + max(0, (s.n + TK - 1) / TK - s.mf);
   return s;
 }
 
-__device__ inline Span span_of_row(const PagedDecodeArgs& a, int b) {
-  const int n = min(max(a.lengths[b], 0), a.W << a.psl);  // W * ps < 2^31 (checked by the launcher)
-  return span_of(n, a.text_len ? a.text_len[b] : 0, a.window, a.sinks);
-}
+// Tiles of one split: the sequence's own, in equal parts of PD_CHUNK tiles at least.
+constexpr int PD_CHUNK = 8;
+__device__ inline int split_tiles(int tt, int nsplit) { return nsplit == 1 ? max(tt, 1) : max(PD_CHUNK, (tt + nsplit - 1) / nsplit); }
 
 }  // namespace
 
@@ -120,141 +125,153 @@ __device__ inline void pd_load_words(unsigned (&dst)[N], const void* src) {  // 
   }
 }
 
-template <int KV, int VW>
-struct PdTile {  // 32 keys: K fragments of both 16-key tiles, and this lane's VW words of each of its 8 V rows
-  pc_u32x4 k[2][KV];
-  unsigned v[8][VW];
-};
-
-template <typename T, int DHT, int NW, bool MASS>
-__global__ __launch_bounds__(NW * 64) void paged_decode_kernel(PagedDecodeArgs a) {
+template <typename T, int DHT, int NW, bool WHOLE>  // WHOLE: dh == DHT, no lane is ever outside the head
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(PagedDecodeArgs a) {
   constexpr bool BF = sizeof(T) == 2;
-  constexpr int DPL = DHT / 16;           // head elements per lane of a V row
-  constexpr int KV = BF ? DHT / 32 : DHT / 16;  // 16-byte K vectors per lane and 16-key tile
-  constexpr int KE = BF ? 8 : 4;          // elements per such vector
-  constexpr int VW = DPL * (int)sizeof(T) / 4;  // 32-bit words per lane of a V row
-  using Tile = PdTile<KV, VW>;
-  extern __shared__ float sm[];  // [NW][ng][DHT] partial outputs, then [NW][16][2] (m, l)
+  constexpr int TK = pc_tile<T>(), ST = TK / 16;  // 16-key score tiles of a step
+  constexpr int DPL = DHT / 16;                   // head elements per lane of a V row
+  constexpr int KV = BF ? DHT / 32 : DHT / 16;    // 16-byte K vectors per lane and score tile
+  constexpr int KE = BF ? 8 : 4;                  // elements per such vector
+  constexpr int VW = DPL * (int)sizeof(T) / 4;    // 32-bit words per lane of a V row
+  extern __shared__ float sm[];  // [NW][ng][DHT] outputs, [NW][16][2] (m, l), [16][2] (m, 1 / l), [ng][score_lds] scores
 
   const int split = blockIdx.x, b = blockIdx.z;
   const int kvh = (int)blockIdx.y / a.GT, gt = (int)blockIdx.y - kvh * a.GT;
   const int h0 = kvh * a.G + gt * 16, ng = min(16, a.G - gt * 16);
-  const Span sp = span_of_row(a, b);
-  const int t0 = split * a.chunk, t1 = min(t0 + a.chunk, sp.tt);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int H = a.Hkv * a.G, ps = 1 << a.psl, dh = a.dh;
+  const Span<TK> sp = span_of_row<TK>(a, b);
+  const int chunk = split_tiles(sp.tt, a.nsplit), t0 = split * chunk, t1 = min(t0 + chunk, sp.tt);
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform, and with it everything about a step but the lanes' own places
+  const int H = a.Hkv * a.G, ps = 1 << a.psl, dh = WHOLE ? DHT : a.dh;
   if (split > 0 && t0 >= sp.tt) return;  // nothing of this sequence is left for this split, and the join does not read it
+
+  float* sm_ml = sm + NW * ng * DHT;
+  float* sm_stat = sm_ml + NW * 32;
+  float* sm_score = sm_stat + 32;
+  const int32_t* tab = a.table + (int64_t)b * a.W;
+  // page ids: lane i holds the page of key key0 + i of one step, fetched a step ahead of the keys; -1: not there
+  auto load_ids = [&](int t) -> int {
+    int id = -1;
+    if (t < t1) {
+      const int j = sp.key0(t) + (lane & (TK - 1));
+      if (j < sp.n) id = tab[j >> a.psl];
+    }
+    return (unsigned)id < (unsigned)a.n_pages ? id : -1;
+  };
+  int ids = load_ids(t0 + w);
 
   pc_u32x4 qf[KV];
   {
-    const T* qp = (const T*)a.q + (int64_t)b * a.q_b + (int64_t)(h0 + min(c, ng - 1)) * a.q_h;
+    const T* qp = (const T*)a.q + (int64_t)b * a.q_b + (int64_t)(h0 + min(c, ng - 1)) * a.q_h + g * KE;
 #pragma unroll
     for (int i = 0; i < KV; ++i) {
-      const int e = i * 4 * KE + g * KE;
-      const bool in = c < ng && e < dh;
       qf[i] = pc_u32x4{0u, 0u, 0u, 0u};
-      if (in) qf[i] = *reinterpret_cast<const pc_u32x4*>(qp + e);
+      if (c < ng && (WHOLE || i * 4 * KE + g * KE < dh)) qf[i] = *reinterpret_cast<const pc_u32x4*>(qp + i * 4 * KE);
     }
   }
-
-  const int32_t* tab = a.table + (int64_t)b * a.W;
   const int64_t page_elems = (int64_t)a.Hkv * ps * dh;
   const T* kbase = (const T*)a.k_pages + (int64_t)kvh * ps * dh;
   const T* vbase = (const T*)a.v_pages + (int64_t)kvh * ps * dh;
-  const bool vin = c * DPL < dh;  // dh is a multiple of 8 and DPL of 4: a lane's dims are inside the head or outside it (DPL 8: dh % 8 == 0)
+  const int koff = c * dh + g * KE, voff = 4 * g * dh + c * DPL;
+  const bool vin = WHOLE || c * DPL < dh;  // dh is a multiple of 8: a lane's elements are inside the head or outside it
 
   float m = -INFINITY, l = -0.0f;  // l stays -0 until a visible key was met: a row that sees nothing answers 0, not 0 / 0
   pc_f32x4 o[DPL];
 #pragma unroll
   for (int j = 0; j < DPL; ++j) o[j] = pc_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // page ids: lane i (0 .. 31) holds the page of key key0 + i of one tile, fetched a tile ahead of the keys
-  auto load_ids = [&](int t) -> int {
-    int id = -1;
-    if (t < t1) {
-      const int j = sp.key0(t) + (lane & 31);
-      if (j < sp.n) id = tab[j >> a.psl];
-    }
-    return (unsigned)id < (unsigned)a.n_pages ? id : -1;
-  };
-  auto load_tile = [&](Tile& tl, int t, int ids) {
-    const int k0 = sp.key0(t);
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const int key = k0 + 16 * st + c;
-      const int id = __shfl(ids, 16 * st + c, 64);
-      const T* p = kbase + (int64_t)max(id, 0) * page_elems + (key & (ps - 1)) * dh;
-#pragma unroll
-      for (int i = 0; i < KV; ++i) {
-        const int e = i * 4 * KE + g * KE;
-        tl.k[st][i] = pc_u32x4{0u, 0u, 0u, 0u};
-        if (id >= 0 && e < dh) tl.k[st][i] = *reinterpret_cast<const pc_u32x4*>(p + e);
-      }
-    }
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const int key = k0 + 16 * st + 4 * g;  // four keys of one page (ps >= 8)
-      const int id = __shfl(ids, 16 * st + 4 * g, 64);
-      const T* p = vbase + (int64_t)max(id, 0) * page_elems + (key & (ps - 1)) * dh + c * DPL;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int i = 0; i < VW; ++i) tl.v[4 * st + r][i] = 0;
-        if (id >= 0 && vin && sp.sees(key + r)) pd_load_words(tl.v[4 * st + r], p + r * dh);  // what nobody sees may hold anything, NaN included
-      }
-    }
-  };
-
-  int ids = load_ids(t0 + w);
   for (int t = t0 + w; t < t1; t += NW) {
-    Tile tl;
-    load_tile(tl, t, ids);
-    const int ids_next = load_ids(t + NW);
     const int k0 = sp.key0(t);
-    const int page_a = __shfl(ids, 4 * g, 64), page_b = __shfl(ids, 16 + 4 * g, 64);
-    ids = ids_next;
-    // ---- scores, in units of the exp2 argument ----
-    pc_f32x4 s[2];
-    bool any = false;
+    pc_u32x4 kf[ST][KV];
+    unsigned vf[4 * ST][VW];
+    int page[ST];  // page of keys 4 g + r of each score tile (four keys share one, ps >= 8)
+    // all keys visible and every score tile on one page that is there: uniform bases, no predicates
+    bool plain = (a.psl >= 4) & sp.sees_tile(k0);
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
+    for (int st = 0; st < ST; ++st) {
+      page[st] = __shfl(ids, 16 * st + 4 * g, 64);
+      plain = plain & (__builtin_amdgcn_readlane(ids, 16 * st) >= 0);
+    }
+    if (plain) {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int64_t at = (int64_t)__builtin_amdgcn_readlane(ids, 16 * st) * page_elems + ((k0 + 16 * st) & (ps - 1)) * dh;
+#pragma unroll
+        for (int i = 0; i < KV; ++i) {
+          if (!WHOLE) kf[st][i] = pc_u32x4{0u, 0u, 0u, 0u};
+          if (WHOLE || i * 4 * KE + g * KE < dh) kf[st][i] = *reinterpret_cast<const pc_u32x4*>(kbase + at + koff + i * 4 * KE);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (!WHOLE) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) vf[4 * st + r][i] = 0;
+          }
+          if (vin) pd_load_words(vf[4 * st + r], vbase + at + voff + r * dh);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int id = __shfl(ids, 16 * st + c, 64), key = k0 + 16 * st + c;
+        const T* p = kbase + (int64_t)max(id, 0) * page_elems + (key & (ps - 1)) * dh + g * KE;
+#pragma unroll
+        for (int i = 0; i < KV; ++i) {
+          kf[st][i] = pc_u32x4{0u, 0u, 0u, 0u};
+          if (id >= 0 && (WHOLE || i * 4 * KE + g * KE < dh)) kf[st][i] = *reinterpret_cast<const pc_u32x4*>(p + i * 4 * KE);
+        }
+        const int k4 = k0 + 16 * st + 4 * g;
+        const T* pv = vbase + (int64_t)max(page[st], 0) * page_elems + (k4 & (ps - 1)) * dh + c * DPL;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int i = 0; i < VW; ++i) vf[4 * st + r][i] = 0;
+          if ((page[st] >= 0) & vin & sp.sees(k4 + r)) pd_load_words(vf[4 * st + r], pv + r * dh);  // what nobody sees may hold anything, NaN included
+        }
+      }
+    }
+    ids = load_ids(t + NW);
+    // ---- scores, in units of the exp2 argument ----
+    pc_f32x4 s[ST];
+    bool any = plain;
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
       s[st] = pc_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KV; ++i) {
         if constexpr (BF) {
-          s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pc_bf16x8, tl.k[st][i]), __builtin_bit_cast(pc_bf16x8, qf[i]), s[st], 0, 0, 0);
+          s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pc_bf16x8, kf[st][i]), __builtin_bit_cast(pc_bf16x8, qf[i]), s[st], 0, 0, 0);
         } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) s[st] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(tl.k[st][i][u]), __uint_as_float(qf[i][u]), s[st], 0, 0, 0);
+          for (int u = 0; u < 4; ++u) s[st] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[st][i][u]), __uint_as_float(qf[i][u]), s[st], 0, 0, 0);
         }
       }
-      const bool there = (st ? page_b : page_a) >= 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
 #pragma clang fp contract(off)  // the rounded product: its difference to the maximum must be 0 for the largest, whatever its size
-        const bool vis = there && sp.sees(k0 + 16 * st + 4 * g + r);
+        const bool vis = plain | ((page[st] >= 0) & sp.sees(k0 + 16 * st + 4 * g + r));
         any |= vis;
-        s[st][r] = vis ? s[st][r] * a.sl2 : -INFINITY;
+        const float x = s[st][r] * a.sl2;
+        s[st][r] = vis ? x : -INFINITY;
       }
     }
-    if constexpr (MASS) {
-      if (c < ng) {
-        float* sc = a.scores + ((int64_t)b * H + h0 + c) * a.score_ld + (int64_t)t * PC_TILE + 4 * g;
-        *reinterpret_cast<pc_f32x4*>(sc) = s[0];
-        *reinterpret_cast<pc_f32x4*>(sc + 16) = s[1];
-      }
+    if (a.mass != nullptr && c < ng) {
+      float* sc = a.score_lds ? sm_score + c * a.score_lds + t * TK + 4 * g : a.scores + ((int64_t)b * H + h0 + c) * a.score_ld + (int64_t)t * TK + 4 * g;
+#pragma unroll
+      for (int st = 0; st < ST; ++st) *reinterpret_cast<pc_f32x4*>(sc + 16 * st) = s[st];
     }
     if (!__any(any)) continue;
     // ---- online softmax of column c ----
-    float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    float mt = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    if constexpr (ST == 2) mt = fmaxf(mt, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mt = rows4_max(mt);
     const float mn = fmaxf(m, mt);
     const float ref = mn == -INFINITY ? 0.f : mn;  // every score so far is -inf: their weights are 0, not exp(-inf + inf)
     const float alpha = __builtin_amdgcn_exp2f(m - ref);
     m = mn;
-    float p[8], sum = 0.f;
+    float p[4 * ST], sum = 0.f;
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+    for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         p[4 * st + r] = __builtin_amdgcn_exp2f(s[st][r] - ref);
@@ -278,22 +295,20 @@ __global__ __launch_bounds__(NW * 64) void paged_decode_kernel(PagedDecodeArgs a
       for (int j = 0; j < DPL; ++j) {
         pc_u32x4 f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[i] = __builtin_amdgcn_perm(tl.v[2 * i + 1][j >> 1], tl.v[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+        for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_perm(vf[2 * i + 1][j >> 1], vf[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
         o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pc_bf16x8, f), hi, o[j], 0, 0, 0);
         o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pc_bf16x8, f), lo, o[j], 0, 0, 0);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4 * ST; ++i)
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(tl.v[i][j]), p[i], o[j], 0, 0, 0);
+        for (int j = 0; j < DPL; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[i][j]), p[i], o[j], 0, 0, 0);
     }
   }
 
   // ---- the waves' parts meet in LDS ----
   l = rows4_sum(l);
-  float* sm_ml = sm + NW * ng * DHT;
   if (c < ng) {
     float* so = sm + (w * ng + c) * DHT;
 #pragma unroll
@@ -306,109 +321,157 @@ __global__ __launch_bounds__(NW * 64) void paged_decode_kernel(PagedDecodeArgs a
     }
   }
   __syncthreads();
-  for (int idx = tid; idx < ng * DHT; idx += NW * 64) {
-    const int hh = idx / DHT, e = idx - hh * DHT;
-    if (e >= dh) continue;
-    float M = -INFINITY;
+  if (tid < ng) {  // one head each: (m, l) over the waves; sm_ml[w][h][0] becomes wave w's factor
+    float M = -INFINITY, L = -0.0f;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, sm_ml[(i * 16 + hh) * 2]);
+    for (int i = 0; i < NW; ++i) M = fmaxf(M, sm_ml[(i * 16 + tid) * 2]);
     const float ref = M == -INFINITY ? 0.f : M;
-    float L = -0.0f, O = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      const float f = __builtin_amdgcn_exp2f(sm_ml[(i * 16 + hh) * 2] - ref);
-      L += sm_ml[(i * 16 + hh) * 2 + 1] * f;
-      O += sm[(i * ng + hh) * DHT + e] * f;
+      const float f = __builtin_amdgcn_exp2f(sm_ml[(i * 16 + tid) * 2] - ref);
+      L += sm_ml[(i * 16 + tid) * 2 + 1] * f;
+      sm_ml[(i * 16 + tid) * 2] = f;
     }
-    if (a.nsplit == 1) store_elem<T>((T*)a.out + ((int64_t)b * H + h0 + hh) * dh + e, __float_as_uint(L) == 0x80000000u ? 0.f : O / L);
-    else a.part_o[(((int64_t)b * H + h0 + hh) * a.nsplit + split) * dh + e] = O;
-    if (e == 0 && a.part_ml != nullptr) {
-      float* ml = a.part_ml + (((int64_t)b * H + h0 + hh) * a.nsplit + split) * 2;
+    sm_stat[tid * 2] = ref;
+    sm_stat[tid * 2 + 1] = __float_as_uint(L) == 0x80000000u ? 0.f : 1.0f / L;
+    if (a.part_ml != nullptr) {
+      float* ml = a.part_ml + (((int64_t)b * H + h0 + tid) * a.nsplit + split) * 2;
       ml[0] = M;
       ml[1] = L;
     }
   }
+  __syncthreads();
+  for (int idx = tid; idx < ng * DHT; idx += NW * 64) {
+    const int hh = idx / DHT, e = idx - hh * DHT;
+    if (!WHOLE && e >= dh) continue;
+    float O = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) O += sm[(i * ng + hh) * DHT + e] * sm_ml[(i * 16 + hh) * 2];
+    if (a.nsplit == 1) store_elem<T>((T*)a.out + ((int64_t)b * H + h0 + hh) * dh + e, O * sm_stat[hh * 2 + 1]);
+    else a.part_o[(((int64_t)b * H + h0 + hh) * a.nsplit + split) * dh + e] = O;
+  }
+  if (a.score_lds == 0) return;
+  for (int idx = tid; idx < sp.tt * TK; idx += NW * 64) {  // the weights of this workgroup's keys and heads
+    const int j = sp.key0(idx / TK) + idx % TK;
+    if (!sp.sees(j)) continue;
+    const int id = tab[j >> a.psl];
+    if ((unsigned)id >= (unsigned)a.n_pages) continue;
+    float sum = 0.f;
+    for (int h = 0; h < ng; ++h) sum += __builtin_amdgcn_exp2f(sm_score[h * a.score_lds + idx] - sm_stat[h * 2]) * sm_stat[h * 2 + 1];
+    // an atomic, because sequences may share the pages of a common prefix; without sharing there is one addend and one result
+    unsafeAtomicAdd(a.mass + ((int64_t)id * a.Hkv + kvh) * ps + (j & (ps - 1)), sum);
+  }
 }
 
-// Joins the splits (blockIdx.x == 0, when there are several) and adds every visible key's weight to `mass` (blockIdx.x >= 1, 1024 keys each).
-constexpr int PD_JOIN_KEYS = 1024, PD_MAX_GROUP = 256;
+// Joins the splits and adds up the weights where a workgroup could not do it alone.  blockIdx.x < a.join_heads: one query head's output; behind them
+// PD_JOIN_KEYS keys each of the weights.
+constexpr int PD_JOIN_KEYS = 1024, PD_MAX_GROUP = 256, PD_MAX_SPLIT = 256;
 
 template <typename T>
 __global__ __launch_bounds__(256) void paged_decode_join_kernel(PagedDecodeArgs a) {
-  __shared__ float sh_m[PD_MAX_GROUP], sh_i[PD_MAX_GROUP];
-  const int b = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x;
-  const int H = a.Hkv * a.G, ps = 1 << a.psl;
-  const Span sp = span_of_row(a, b);
-  const int used = max(1, (sp.tt + a.chunk - 1) / a.chunk);
-  const int part = (int)blockIdx.x - (a.nsplit > 1 ? 1 : 0);  // -1: the outputs
-  if (part >= 0 && part * PD_JOIN_KEYS >= sp.tt * PC_TILE) return;
-  for (int h = tid; h < a.G; h += 256) {  // the statistics of the group's heads over all splits
-    const float* ml = a.part_ml + ((int64_t)b * H + kvh * a.G + h) * a.nsplit * 2;
+  constexpr int TK = pc_tile<T>();
+  __shared__ float sh_a[256], sh_b[256];
+  __shared__ float sh_o[256 * 4];
+  const int b = blockIdx.z, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int H = a.Hkv * a.G, ps = 1 << a.psl, dh = a.dh;
+  const Span<TK> sp = span_of_row<TK>(a, b);
+  const int chunk = split_tiles(sp.tt, a.nsplit), used = max(1, (sp.tt + chunk - 1) / chunk);
+  // (reference, 1 / sum) of one head over its splits, by one wave
+  auto stats = [&](const float* ml, float& ref, float& inv) {
     float M = -INFINITY, L = -0.0f;
-    for (int s = 0; s < used; ++s) M = fmaxf(M, ml[2 * s]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < used; ++s) L += ml[2 * s + 1] * __builtin_amdgcn_exp2f(ml[2 * s] - ref);
-    sh_m[h] = ref;
-    sh_i[h] = __float_as_uint(L) == 0x80000000u ? 0.f : 1.0f / L;
-  }
-  __syncthreads();
-  if (part < 0) {
-    for (int idx = tid; idx < a.G * a.dh; idx += 256) {
-      const int h = idx / a.dh, e = idx - h * a.dh;
-      const int64_t hb = (int64_t)b * H + kvh * a.G + h;
-      float O = 0.f;
-      for (int s = 0; s < used; ++s) O += a.part_o[(hb * a.nsplit + s) * a.dh + e] * __builtin_amdgcn_exp2f(a.part_ml[(hb * a.nsplit + s) * 2] - sh_m[h]);
-      store_elem<T>((T*)a.out + hb * a.dh + e, O * sh_i[h]);
+    for (int s = lane; s < used; s += 64) M = fmaxf(M, ml[2 * s]);
+    M = wave_max(M);
+    ref = M == -INFINITY ? 0.f : M;
+    for (int s = lane; s < used; s += 64) L += ml[2 * s + 1] * __builtin_amdgcn_exp2f(ml[2 * s] - ref);
+    L = wave_sum(L);
+    inv = __float_as_uint(L) == 0x80000000u ? 0.f : 1.0f / L;
+  };
+  if ((int)blockIdx.x < a.join_heads) {
+    const int64_t hb = (int64_t)b * H + kvh * a.G + blockIdx.x;
+    const float* ml = a.part_ml + hb * a.nsplit * 2;
+    float ref, inv;
+    stats(ml, ref, inv);
+    if (tid < used) sh_a[tid] = __builtin_amdgcn_exp2f(ml[2 * tid] - ref);
+    __syncthreads();
+    // dh / 4 threads a row of partial outputs, 256 / (dh / 4) rows at a time
+    const int vpr = dh / 4, rows = 256 / vpr, e = (tid % vpr) * 4, r0 = tid / vpr;
+    pc_f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    if (r0 < rows)
+      for (int s = r0; s < used; s += rows) O += *reinterpret_cast<const pc_f32x4*>(a.part_o + (hb * a.nsplit + s) * dh + e) * sh_a[s];
+    *reinterpret_cast<pc_f32x4*>(sh_o + tid * 4) = O;
+    __syncthreads();
+    for (int i = tid; i < dh; i += 256) {
+      float sum = 0.f;
+      for (int r = 0; r < rows; ++r) sum += sh_o[r * vpr * 4 + i];
+      store_elem<T>((T*)a.out + hb * dh + i, sum * inv);
     }
     return;
   }
-  for (int idx = part * PD_JOIN_KEYS + tid; idx < min((part + 1) * PD_JOIN_KEYS, sp.tt * PC_TILE); idx += 256) {
-    const int j = sp.key0(idx / PC_TILE) + idx % PC_TILE;
+  const int part = (int)blockIdx.x - a.join_heads;
+  if (part * PD_JOIN_KEYS >= sp.tt * TK) return;
+  for (int h = w; h < a.G; h += 4) {
+    float ref, inv;
+    stats(a.part_ml + ((int64_t)b * H + kvh * a.G + h) * a.nsplit * 2, ref, inv);
+    if (lane == 0) {
+      sh_a[h] = ref;
+      sh_b[h] = inv;
+    }
+  }
+  __syncthreads();
+  for (int idx = part * PD_JOIN_KEYS + tid; idx < min((part + 1) * PD_JOIN_KEYS, sp.tt * TK); idx += 256) {
+    const int j = sp.key0(idx / TK) + idx % TK;
     if (!sp.sees(j)) continue;
     const int page = a.table[(int64_t)b * a.W + (j >> a.psl)];
     if ((unsigned)page >= (unsigned)a.n_pages) continue;
     const float* sc = a.scores + ((int64_t)b * H + kvh * a.G) * a.score_ld + idx;
     float sum = 0.f;
-    for (int h = 0; h < a.G; ++h) sum += __builtin_amdgcn_exp2f(sc[h * a.score_ld] - sh_m[h]) * sh_i[h];
-    // an atomic, because sequences may share the pages of a common prefix; without sharing there is one addend and one result
+    for (int h = 0; h < a.G; ++h) sum += __builtin_amdgcn_exp2f(sc[h * a.score_ld] - sh_a[h]) * sh_b[h];
     unsafeAtomicAdd(a.mass + ((int64_t)page * a.Hkv + kvh) * ps + (j & (ps - 1)), sum);
   }
 }
 
-static int pd_tiles_bound(int W, int ps, int window, int sinks, bool text) {  // tiles of a sequence, at most
+static int pd_tiles_bound(int W, int ps, int window, int sinks, bool text, int tk) {  // tiles of a sequence, at most
   const int64_t n = (int64_t)W * ps;
-  const int full = (int)((n + PC_TILE - 1) / PC_TILE);
+  const int full = (int)((n + tk - 1) / tk);
   if (window <= 0 || window >= n || text) return full;
-  return (int)std::min((int64_t)full, ((int64_t)sinks + PC_TILE - 1) / PC_TILE + ((int64_t)window + PC_TILE - 1) / PC_TILE + 1);
+  return (int)std::min((int64_t)full, ((int64_t)sinks + tk - 1) / tk + ((int64_t)window + tk - 1) / tk + 1);
 }
 
-PagedDecodePlan paged_decode_plan(int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass) {
+PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass) {
   PagedDecodePlan p;
-  const int tiles = std::max(1, pd_tiles_bound(W, ps, window, sinks, text));
-  const int64_t groups = (int64_t)B * Hkv * ((G + 15) / 16);
-  p.tiles = tiles;
-  p.nw = 4;
-  p.chunk = tiles;
+  const int tk = dtype == DT_F32 ? 16 : 32, ng = std::min(16, G);
+  p.tiles = std::max(1, pd_tiles_bound(W, ps, window, sinks, text, tk));
+  const int64_t groups = (int64_t)B * Hkv * ((G + 15) / 16), H = (int64_t)Hkv * G;
   p.nsplit = 1;
-  if (groups < 512 && tiles > 16) {
-    p.chunk = (int)std::max((int64_t)16, (tiles * groups + 1023) / 1024);
-    p.nsplit = (tiles + p.chunk - 1) / p.chunk;
+  p.nw = groups < 512 && ng <= 8 ? 8 : 4;  // 8 waves: their outputs fit 32 KB of LDS for up to 8 heads
+  if (groups < 512 && p.tiles > 8 * p.nw) {
+    p.nw = 4;
+    p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), (3072 + groups - 1) / groups);
   }
-  const int64_t H = (int64_t)Hkv * G;
-  p.ml_floats = (p.nsplit > 1 || mass) ? (size_t)(B * H * p.nsplit * 2) : 0;
+  // weights: by the workgroup that has all of a head's scores, where they fit beside its outputs; else by the join
+  p.score_lds = mass && p.nsplit == 1 && G <= 16 && (int64_t)p.tiles * tk * ng <= 7168 ? p.tiles * tk : 0;
+  const bool join_mass = mass && p.score_lds == 0;
+  p.ml_floats = (p.nsplit > 1 || join_mass) ? (size_t)(B * H * p.nsplit * 2) : 0;
   p.o_floats = p.nsplit > 1 ? (size_t)(B * H * p.nsplit * dh) : 0;
-  p.score_floats = mass ? (size_t)(B * H) * tiles * PC_TILE : 0;
+  p.score_floats = join_mass ? (size_t)(B * H) * p.tiles * tk : 0;
   return p;
 }
 
-template <typename T, int DHT>
-static int pd_launch(hipStream_t st, const PagedDecodePlan& p, const PagedDecodeArgs& a, int B) {
+template <typename T, int DHT, int NW>
+static void pd_launch_nw(hipStream_t st, const PagedDecodePlan& p, const PagedDecodeArgs& a, int B) {
   const int ng = std::min(16, a.G);
-  const size_t lds = ((size_t)p.nw * ng * DHT + p.nw * 32) * sizeof(float);
-  const dim3 grid(p.nsplit, a.Hkv * a.GT, B), block(p.nw * 64);
-  if (a.mass != nullptr) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, 4, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, 4, false>), grid, block, lds, st, a);
-  const int parts = (p.nsplit > 1 ? 1 : 0) + (a.mass != nullptr ? (p.tiles * PC_TILE + PD_JOIN_KEYS - 1) / PD_JOIN_KEYS : 0);
+  const size_t lds = ((size_t)NW * ng * DHT + NW * 32 + 32 + (size_t)ng * p.score_lds) * sizeof(float);
+  const dim3 grid(p.nsplit, a.Hkv * a.GT, B), block(NW * 64);
+  if (a.dh == DHT) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, false>), grid, block, lds, st, a);
+}
+
+template <typename T, int DHT>
+static int pd_launch(hipStream_t st, const PagedDecodePlan& p, PagedDecodeArgs& a, int B) {
+  if (p.nw == 8) pd_launch_nw<T, DHT, 8>(st, p, a, B);
+  else pd_launch_nw<T, DHT, 4>(st, p, a, B);
+  a.join_heads = p.nsplit > 1 ? a.G : 0;
+  const int parts = a.join_heads + (p.score_floats ? (p.tiles * pc_tile<T>() + PD_JOIN_KEYS - 1) / PD_JOIN_KEYS : 0);
   if (parts > 0) hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(parts, a.Hkv, B), dim3(256), 0, st, a);
   return 0;
 }
@@ -417,9 +480,9 @@ int launch_paged_decode(hipStream_t st, int dtype, const PagedDecodePlan& p, Pag
   if (B <= 0) return 0;
   if (a.G > PD_MAX_GROUP) return -1;
   a.GT = (a.G + 15) / 16;
-  a.chunk = p.chunk;
   a.nsplit = p.nsplit;
-  a.score_ld = (int64_t)p.tiles * PC_TILE;
+  a.score_lds = p.score_lds;
+  a.score_ld = (int64_t)p.tiles * (dtype == DT_F32 ? 16 : 32);
   if (dtype == DT_F32) return a.dh <= 64 ? pd_launch<float, 64>(st, p, a, B) : pd_launch<float, 128>(st, p, a, B);
   return a.dh <= 64 ? pd_launch<bf16_t, 64>(st, p, a, B) : pd_launch<bf16_t, 128>(st, p, a, B);
 }
@@ -448,9 +511,12 @@ __device__ inline EvictRow evict_row(const EvictArgs& a, int b) {
   return r;
 }
 
+// KPT > 0: the keys of up to EV_T * KPT candidates stay in registers; KPT = 0: any number, read again in every pass.
+template <int KPT>
 __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
-  __shared__ int bins[EV_BINS];
+  __shared__ int bins[3][EV_BINS];
   __shared__ int wsum[EV_NW], wsum2[EV_NW];
+  __shared__ int cnt[2][(KPT > 0 ? KPT : 1) * EV_NW];
   __shared__ int sh_bin, sh_above;
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, ps = 1 << a.psl;
   const EvictRow r = evict_row(a, b);
@@ -460,29 +526,39 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
     for (int i = tid; i < a.budget; i += EV_T) kept[i] = i < r.n ? i : -1;
     return;
   }
-  for (int i = tid; i < r.S; i += EV_T) kept[i] = i;
-  for (int i = tid; i < r.R; i += EV_T) kept[r.S + r.M + i] = r.n - r.R + i;
-  if (r.M == 0) return;
-  const int C = r.n - r.S - r.R;  // > M >= 1
+  const int C = r.n - r.S - r.R;  // > M
   const int32_t* tab = a.table + (int64_t)b * a.W;
   auto weight = [&](int i) -> uint32_t {  // key of candidate i; the keys of a page that is not there have no weight
     const int j = r.S + i, page = tab[j >> a.psl];
     return (unsigned)page < (unsigned)a.n_pages ? ev_key(a.mass[((int64_t)page * a.Hkv + h) * ps + (j & (ps - 1))]) : ev_key(0.f);
   };
+  uint32_t key[KPT > 0 ? KPT : 1];
+#pragma unroll
+  for (int u = 0; u < KPT; ++u) key[u] = u * EV_T + tid < C ? weight(u * EV_T + tid) : 0u;
+  for (int i = tid; i < r.S; i += EV_T) kept[i] = i;
+  for (int i = tid; i < r.R; i += EV_T) kept[r.S + r.M + i] = r.n - r.R + i;
+  if (r.M == 0) return;
+  for (int i = tid; i < 3 * EV_BINS; i += EV_T) (&bins[0][0])[i] = 0;
+  __syncthreads();
   uint32_t prefix = 0, have = 0;  // the bits of the M-th largest key that are known, and their mask
   int need = r.M;                 // its rank among the keys that agree with them
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, nb = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < EV_BINS; i += EV_T) bins[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < C; i += EV_T) {
-      const uint32_t k = weight(i);
-      if ((k & have) == prefix) atomicAdd(&bins[(k >> shift) & (nb - 1)], 1);
+    int* bin = bins[pass];
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int u = 0; u < KPT; ++u)
+        if (u * EV_T + tid < C && (key[u] & have) == prefix) atomicAdd(&bin[(key[u] >> shift) & (nb - 1)], 1);
+    } else {
+      for (int i = tid; i < C; i += EV_T) {
+        const uint32_t k = weight(i);
+        if ((k & have) == prefix) atomicAdd(&bin[(k >> shift) & (nb - 1)], 1);
+      }
     }
     __syncthreads();
     // thread t counts bins 2047 - 2 t and 2046 - 2 t: an inclusive scan from the top finds the bin the need-th largest falls into
-    const int hi = bins[EV_BINS - 1 - 2 * tid], lo = bins[EV_BINS - 2 - 2 * tid];
+    const int hi = bin[EV_BINS - 1 - 2 * tid], lo = bin[EV_BINS - 2 - 2 * tid];
     int inc = hi + lo;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -492,7 +568,8 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
     if (lane == 63) wsum[w] = inc;
     __syncthreads();
     int before = inc - hi - lo;
-    for (int i = 0; i < w; ++i) before += wsum[i];
+#pragma unroll
+    for (int i = 0; i < EV_NW; ++i) before += i < w ? wsum[i] : 0;
     if (before < need && need <= before + hi) {
       sh_bin = EV_BINS - 1 - 2 * tid;
       sh_above = before;
@@ -504,86 +581,173 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
     prefix |= (uint32_t)sh_bin << shift;
     have |= (uint32_t)(nb - 1) << shift;
     need -= sh_above;
-    __syncthreads();
   }
   // every key above `prefix` stays, and of those equal to it the first `need`
-  int run = 0, run_eq = 0;
-  for (int i0 = 0; i0 < C; i0 += EV_T) {
-    const int i = i0 + tid;
-    const uint32_t k = i < C ? weight(i) : 0u;
-    const bool eq = i < C && k == prefix, gt = i < C && k > prefix;
-    const unsigned long long beq = __ballot(eq), bgt = __ballot(gt), below = (1ull << lane) - 1;
-    if (lane == 0) {
-      wsum[w] = __popcll(beq);
-      wsum2[w] = __popcll(bgt);
-    }
-    __syncthreads();
-    int eq_before = run_eq + __popcll(beq & below), gt_before = run + __popcll(bgt & below), eq_all = 0, gt_all = 0;
-#pragma unroll
-    for (int q = 0; q < EV_NW; ++q) {
-      eq_before += q < w ? wsum[q] : 0;
-      gt_before += q < w ? wsum2[q] : 0;
-      eq_all += wsum[q];
-      gt_all += wsum2[q];
-    }
+  const unsigned long long below = (1ull << lane) - 1;
+  auto keep = [&](int i, bool gt, bool eq, int gt_before, int eq_before) {
     const int at = gt_before + min(eq_before, need);
     if ((gt || (eq && eq_before < need)) && at < r.M) kept[r.S + at] = r.S + i;  // at < M always, unless the weights change during the call
-    run += gt_all;
-    run_eq += eq_all;
+  };
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+      const bool in = u * EV_T + tid < C;
+      const unsigned long long beq = __ballot(in && key[u] == prefix), bgt = __ballot(in && key[u] > prefix);
+      if (lane == 0) {
+        cnt[0][u * EV_NW + w] = __popcll(bgt);
+        cnt[1][u * EV_NW + w] = __popcll(beq);
+      }
+    }
     __syncthreads();
+    if (w < 2) {  // exclusive scan of each list by one wave, in the order of the positions
+      constexpr int PER = (KPT * EV_NW + 63) / 64;
+      int v[PER], sum = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        v[i] = lane * PER + i < KPT * EV_NW ? cnt[w][lane * PER + i] : 0;
+        sum += v[i];
+      }
+      int inc = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += t;
+      }
+      inc -= sum;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (lane * PER + i < KPT * EV_NW) cnt[w][lane * PER + i] = inc;
+        inc += v[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+      const int i = u * EV_T + tid;
+      const bool eq = i < C && key[u] == prefix, gt = i < C && key[u] > prefix;
+      const unsigned long long beq = __ballot(eq), bgt = __ballot(gt);
+      keep(i, gt, eq, cnt[0][u * EV_NW + w] + __popcll(bgt & below), cnt[1][u * EV_NW + w] + __popcll(beq & below));
+    }
+  } else {
+    int run = 0, run_eq = 0;
+    for (int i0 = 0; i0 < C; i0 += EV_T) {
+      const int i = i0 + tid;
+      const uint32_t k = i < C ? weight(i) : 0u;
+      const bool eq = i < C && k == prefix, gt = i < C && k > prefix;
+      const unsigned long long beq = __ballot(eq), bgt = __ballot(gt);
+      if (lane == 0) {
+        wsum[w] = __popcll(beq);
+        wsum2[w] = __popcll(bgt);
+      }
+      __syncthreads();
+      int eq_before = run_eq + __popcll(beq & below), gt_before = run + __popcll(bgt & below);
+#pragma unroll
+      for (int q = 0; q < EV_NW; ++q) {
+        eq_before += q < w ? wsum[q] : 0;
+        gt_before += q < w ? wsum2[q] : 0;
+        run_eq += wsum[q];
+        run += wsum2[q];
+      }
+      keep(i, gt, eq, gt_before, eq_before);
+      __syncthreads();
+    }
   }
 }
 
-// The keys that stay move up in place: row i takes the place of kept[i] >= i.  Rows are moved in ascending chunks by ONE workgroup per (sequence,
-// head, K | V | weights): a chunk's targets lie below every later chunk's sources, so only the rows of one chunk can overwrite each other's
-// sources, and a barrier between a chunk's loads and its stores rules that out.
-constexpr int MV_T = 256, MV_U = 8;
+// The keys that stay move up in place: row i takes the place of kept[i] >= i.  Rows move in ascending chunks, all of a head's columns of one pool
+// (or a slice of them) by ONE workgroup: a chunk's targets lie below every later chunk's sources, so the next chunk may be on its way while this
+// one is stored, and only the rows of one chunk can overwrite each other's sources -- a barrier between its loads' return and its stores rules
+// that out.  HBM-bound; two chunks of 8 vectors per thread in flight.
+constexpr int MV_T = 256, MV_U = 8, MV_TAB = 4096;
 
 template <typename V>
-__device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* kept, const int32_t* tab, int h, int vpr, int n, int len) {
-  const int tid = threadIdx.x, ps = 1 << a.psl;
+__device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* kept, const int32_t* tab, const int32_t* sh_tab, int h, int vpr, int e0,
+                                  int width, int len) {
+  const int tid = threadIdx.x, ps = 1 << a.psl, n = a.budget;
   const int64_t page_vecs = (int64_t)a.Hkv * ps * vpr;
-  const int total = n * vpr;  // vectors
-  for (int i0 = 0; i0 < total; i0 += MV_T * MV_U) {
-    V x[MV_U];
-    V* dst[MV_U];
+  const int rows = MV_T / width, row0 = tid / width, e = e0 + tid % width;  // rows a pass, this thread's and its column
+  const bool mine = row0 < rows;
+  auto page_of = [&](int j) { return sh_tab != nullptr ? sh_tab[j >> a.psl] : tab[j >> a.psl]; };
+  int from[MV_U];
+  auto load_kept = [&](int base) {
 #pragma unroll
     for (int u = 0; u < MV_U; ++u) {
-      const int i = i0 + u * MV_T + tid;
+      const int row = base + u * rows + row0;
+      from[u] = mine && row < n ? kept[row] : -1;
+    }
+  };
+  // loads are unconditional (from the pool's first vector where there is nothing to move), so that the waits for them can be counted
+  auto load_rows = [&](int base, V (&x)[MV_U], V* (&dst)[MV_U]) {
+#pragma unroll
+    for (int u = 0; u < MV_U; ++u) {
+      const int row = base + u * rows + row0;
+      const V* src = pool;
       dst[u] = nullptr;
-      if (i < total) {
-        const int row = i / vpr, e = i - row * vpr, from = kept[row];
-        if (from != row && (unsigned)from < (unsigned)len) {
-          const int sp = tab[from >> a.psl], dp = tab[row >> a.psl];
-          if ((unsigned)sp < (unsigned)a.n_pages && (unsigned)dp < (unsigned)a.n_pages) {
-            x[u] = pool[(int64_t)sp * page_vecs + (int64_t)(h * ps + (from & (ps - 1))) * vpr + e];
-            dst[u] = pool + (int64_t)dp * page_vecs + (int64_t)(h * ps + (row & (ps - 1))) * vpr + e;
-          }
+      if (from[u] > row && from[u] < len) {
+        const int sp = page_of(from[u]), dp = page_of(row);
+        if ((unsigned)sp < (unsigned)a.n_pages && (unsigned)dp < (unsigned)a.n_pages) {
+          src = pool + (int64_t)sp * page_vecs + (int64_t)(h * ps + (from[u] & (ps - 1))) * vpr + e;
+          dst[u] = pool + (int64_t)dp * page_vecs + (int64_t)(h * ps + (row & (ps - 1))) * vpr + e;
         }
       }
+      x[u] = *src;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the chunk have returned
+  };
+  const int step = MV_U * rows;
+  auto turn = [&](int base, V (&x)[MV_U], V* (&dst)[MV_U], V (&x2)[MV_U], V* (&dst2)[MV_U]) {
+    if (base + step < n) {
+      load_rows(base + step, x2, dst2);
+      load_kept(base + 2 * step);
+    }
+#pragma unroll
+    for (int u = 0; u < MV_U; ++u) asm volatile("" : "+v"(x[u])::"memory");  // the chunk's loads have returned to this wave
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < MV_U; ++u)
       if (dst[u] != nullptr) *dst[u] = x[u];
+  };
+  V x[MV_U], y[MV_U];
+  V *dx[MV_U], *dy[MV_U];
+  load_kept(0);
+  load_rows(0, x, dx);
+  load_kept(step);
+  for (int base = 0; base < n; base += 2 * step) {
+    turn(base, x, dx, y, dy);
+    if (base + step < n) turn(base + step, y, dy, x, dx);
   }
 }
 
-__global__ __launch_bounds__(MV_T) void kv_evict_move_kernel(EvictArgs a, int vpr) {
+// blockIdx.z: 2 * slices parts of the keys and values, then the weights
+__global__ __launch_bounds__(MV_T) void kv_evict_move_kernel(EvictArgs a, int vpr, int slices) {
+  __shared__ int32_t sh_tab[MV_TAB];
   const int h = blockIdx.x, b = blockIdx.y, what = blockIdx.z;
   const EvictRow r = evict_row(a, b);
   if (r.n <= a.budget) return;
   const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
   const int32_t* tab = a.table + (int64_t)b * a.W;
-  if (what == 2) evict_move<float>(a.mass, a, kept, tab, h, 1, a.budget, r.n);
-  else evict_move<pc_u32x4>((pc_u32x4*)(what ? a.v_pages : a.k_pages), a, kept, tab, h, vpr, a.budget, r.n);
+  const int used = (r.n + (1 << a.psl) - 1) >> a.psl;  // pages of the sequence
+  const int32_t* cached = used <= MV_TAB ? sh_tab : nullptr;
+  if (cached != nullptr)
+    for (int i = threadIdx.x; i < used; i += MV_T) sh_tab[i] = tab[i];
+  __syncthreads();
+  if (what == 2 * slices) {
+    evict_move<float>(a.mass, a, kept, tab, cached, h, 1, 0, 1, r.n);
+  } else {
+    const int width = vpr / slices;
+    evict_move<pc_u32x4>((pc_u32x4*)(what < slices ? a.k_pages : a.v_pages), a, kept, tab, cached, h, vpr, (what % slices) * width, width, r.n);
+  }
 }
 
 int launch_kv_evict(hipStream_t st, int dtype, const EvictArgs& a, int B, int dh) {
   if (B <= 0) return 0;
-  hipLaunchKernelGGL(kv_evict_select_kernel, dim3(a.Hkv, B), dim3(EV_T), 0, st, a);
-  hipLaunchKernelGGL(kv_evict_move_kernel, dim3(a.Hkv, B, 3), dim3(MV_T), 0, st, a, dh * (dtype == DT_F32 ? 4 : 2) / 16);
+  const int64_t most = (int64_t)a.W << a.psl;
+  const dim3 sgrid(a.Hkv, B);
+  if (most <= 4 * EV_T) hipLaunchKernelGGL((kv_evict_select_kernel<4>), sgrid, dim3(EV_T), 0, st, a);
+  else if (most <= 16 * EV_T) hipLaunchKernelGGL((kv_evict_select_kernel<16>), sgrid, dim3(EV_T), 0, st, a);
+  else hipLaunchKernelGGL((kv_evict_select_kernel<0>), sgrid, dim3(EV_T), 0, st, a);
+  const int vpr = dh * (dtype == DT_F32 ? 4 : 2) / 16;
+  const int slices = vpr % 8 == 0 ? vpr / 8 : 1;  // whole 128-byte lines of a row each
+  hipLaunchKernelGGL(kv_evict_move_kernel, dim3(a.Hkv, B, 2 * slices + 1), dim3(MV_T), 0, st, a, vpr, slices);
   return 0;
 }
 

@@ -95,9 +95,10 @@ __device__ inline Tiles tiles_of(int i0, int i1, int text, int window, int sinks
 // What one row sees: keys j < hd, and lo <= j <= i.
 struct Sight {
   int hd, lo, i;
-  __device__ bool sees(int j) const { return j < hd || (j >= lo && j <= i); }
-  __device__ bool all(int j0, int n) const { return j0 + n <= hd || (j0 >= lo && j0 + n - 1 <= i); }
-  __device__ bool any(int j0, int n) const { return j0 < hd || (j0 <= i && j0 + n - 1 >= lo); }
+  // (& and | on purpose: a select per key, no branches)
+  __device__ bool sees(int j) const { return (j < hd) | ((j >= lo) & (j <= i)); }
+  __device__ bool all(int j0, int n) const { return (j0 + n <= hd) | ((j0 >= lo) & (j0 + n - 1 <= i)); }
+  __device__ bool any(int j0, int n) const { return (j0 < hd) | ((j0 <= i) & (j0 + n - 1 >= lo)); }
 };
 __device__ inline Sight sight_of(int i, int text, int window, int sinks) {
   Sight s;
@@ -294,11 +295,31 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 #pragma unroll
     for (int f = 0; f < QW; ++f) {
       if (!unmasked) {
+        // tiles behind the head hold no key below hd, and as a rule only one edge of the window: one compare with a constant per score
+        const int hi = see[f].i - kt0 - g * 4, lo = see[f].lo - kt0 - g * 4;  // key number 16 kb4 + r of this lane is visible from lo to hi
+        if (t < ti.th) {
+          const int hd = see[f].hd - kt0 - g * 4;  // or below hd
 #pragma unroll
-        for (int kb4 = 0; kb4 < 4; ++kb4)
+          for (int kb4 = 0; kb4 < 4; ++kb4)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!see[f].sees(kt0 + kb4 * 16 + g * 4 + r)) s[f][kb4][r] = -INFINITY;
+            for (int r = 0; r < 4; ++r)
+              s[f][kb4][r] = (kb4 * 16 + r >= hd) & ((kb4 * 16 + r < lo) | (kb4 * 16 + r > hi)) ? -INFINITY : s[f][kb4][r];
+        } else {
+          if (__any(see[f].i < kt0 + TK - 1)) {
+#pragma unroll
+            for (int kb4 = 0; kb4 < 4; ++kb4)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                s[f][kb4][r] = kb4 * 16 + r > hi ? -INFINITY : s[f][kb4][r];
+          }
+          if (__any(see[f].lo > kt0)) {
+#pragma unroll
+            for (int kb4 = 0; kb4 < 4; ++kb4)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                s[f][kb4][r] = kb4 * 16 + r < lo ? -INFINITY : s[f][kb4][r];
+          }
+        }
       }
       float mt = fmaxf(fmaxf(s[f][0][0], s[f][0][1]), fmaxf(s[f][0][2], s[f][0][3]));
 #pragma unroll
@@ -447,7 +468,7 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if (!unmasked && !see.sees(kt0 + kt * 16 + g * 4 + r)) s[kt][r] = -INFINITY;
+        s[kt][r] = unmasked | see.sees(kt0 + kt * 16 + g * 4 + r) ? s[kt][r] : -INFINITY;
         mt = fmaxf(mt, s[kt][r]);
       }
     mt = rows4_max(mt);

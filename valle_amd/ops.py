@@ -6,10 +6,8 @@ All tensors must live on a ROCm device; nothing here computes on the host.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
-import math
 from typing import Optional
 
 import torch
@@ -381,73 +379,89 @@ def linear_fp8(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scal
 # Row i of a sequence sees key j iff  j < text_len  or  (j <= i and (window == 0 or i - j < window or j < sinks)).
 # Forward only.  What an index tensor holds is not read on the host (no synchronization, every call can be captured into a graph): the kernels
 # clamp offsets and lengths and never follow a page id outside the pool.
-_NO_GUARD = contextlib.nullcontext()
+def _refuse(who: str, what: str):
+    raise ValueError(f"{who}: {what}")
 
 
-def _need(ok: bool, who: str, what: str):
-    if not ok:
-        raise ValueError(f"{who}: {what}")
-
-
-def _operands(who: str, first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """Same device and type, no gradient asked for; -> the dtype code."""
+def _operands(who: str, first: torch.Tensor, *others: torch.Tensor) -> int:
+    """One device, one type, no gradient asked for; -> the type's code."""
     dt = _dt(first)
+    grad = first.requires_grad
+    where, what = first.device, first.dtype
     for t in others:
-        if t is not None and t.dtype != first.dtype:
-            raise TypeError(f"{who}: dtypes {first.dtype} and {t.dtype} differ")
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        if t.dtype != what:
+            raise TypeError(f"{who}: dtypes {what} and {t.dtype} differ")
+        if t.device != where:
+            _refuse(who, "all tensors must be on one device")
+        grad = grad or t.requires_grad
+    if grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who} has no backward pass: detach its operands or call it under torch.no_grad()")
-    for t in others:
-        _need(t is None or t.device == first.device, who, "all tensors must be on one device")
     return dt
 
 
-def _launch_on(t: torch.Tensor):
-    """(stream, guard): the current stream of t's device, and a context that makes that device current where it is not."""
-    st = _st(t)
-    return st, _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
 def _index(who: str, name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor):
+    """Address of an int32 vector of n values on like's device (None: NULL), and the tensor that must outlive the call."""
     if t is None:
-        return None
+        return None, None
     if t.dtype != torch.int32:
         raise TypeError(f"{who}: {name} must be int32, got {t.dtype}")
-    _need(t.dim() == 1 and t.shape[0] == n, who, f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    _need(t.device == like.device, who, f"{name} must be on {like.device}")
-    return t if t.is_contiguous() else t.contiguous()
+    if t.shape != (n,):
+        _refuse(who, f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    if t.device != like.device:
+        _refuse(who, f"{name} must be on {like.device}")
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.data_ptr(), t
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """t (rows, heads, dh) as it is where every row and head starts on 16 bytes, else a contiguous copy."""
-    v = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % v == 0 and t.stride(1) % v == 0 and t.data_ptr() % 16 == 0:
+    v = 8 if t.dtype == torch.bfloat16 else 4
+    r, h, e = t.stride()
+    if e == 1 and r % v == 0 and h % v == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _out(who: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    _need(out.shape == like.shape and out.dtype == like.dtype and out.device == like.device and out.is_contiguous() and out.data_ptr() % 16 == 0,
-          who, "out must be a contiguous tensor like q, on 16 bytes")
+        return like.new_empty(like.shape)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() or out.data_ptr() % 16:
+        _refuse(who, "out must be a contiguous tensor like q, on 16 bytes")
     return out
 
 
 def _pages(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, mass: Optional[torch.Tensor]):
     """Checks of a page pool; -> (n_pages, heads, page size, dh, sequences, table width)."""
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, who, "k_pages and v_pages must have one shape (n_pages, heads, page_size, dh)")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), who, "pages must be contiguous")
+    shape, where = k_pages.shape, k_pages.device
+    if len(shape) != 4 or v_pages.shape != shape:
+        _refuse(who, "k_pages and v_pages must have one shape (n_pages, heads, page_size, dh)")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _refuse(who, "pages must be contiguous")
     if page_table.dtype != torch.int32:
         raise TypeError(f"{who}: page_table must be int32, got {page_table.dtype}")
-    _need(page_table.dim() == 2 and page_table.is_contiguous() and page_table.device == k_pages.device, who,
-          "page_table must be a contiguous (sequences, pages) tensor on the pages' device")
+    if page_table.dim() != 2 or not page_table.is_contiguous() or page_table.device != where:
+        _refuse(who, "page_table must be a contiguous (sequences, pages) tensor on the pages' device")
     if mass is not None:
         if mass.dtype != torch.float32:
             raise TypeError(f"{who}: mass must be float32, got {mass.dtype}")
-        _need(mass.shape == k_pages.shape[:3] and mass.is_contiguous() and mass.device == k_pages.device, who,
-              "mass must be a contiguous (n_pages, heads, page_size) tensor on the pages' device")
-    return (*k_pages.shape, *page_table.shape)
+        if mass.shape != shape[:3] or not mass.is_contiguous() or mass.device != where:
+            _refuse(who, "mass must be a contiguous (n_pages, heads, page_size) tensor on the pages' device")
+    return (*shape, *page_table.shape)
+
+
+def _call(t: torch.Tensor, entry: str, *args) -> None:
+    """A C entry on the current stream of t's device, with that device current."""
+    assert t.is_cuda, "HIP operators need device tensors (no CPU fallback)"
+    i = t.get_device()
+    fn = getattr(_lib.load(), entry)
+    if i == torch._C._cuda_getDevice():
+        rc = fn(torch._C._cuda_getCurrentRawStream(i), *args)
+    else:
+        with torch.cuda.device(i):
+            rc = fn(torch._C._cuda_getCurrentRawStream(i), *args)
+    if rc:
+        _lib.check(rc)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: torch.Tensor, window: int = 0, sinks: int = 0,
@@ -460,22 +474,23 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     holds are 0, or left as they were in a given `out` (which must not overlap the operands).  A key that a row does not see cannot
     reach it, whatever it holds.  No synchronization; forward only."""
     who = "window_attention"
-    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape, who, "q (rows, H, dh), k and v (rows, Hkv, dh)")
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        _refuse(who, "q must be (rows, H, dh), k and v (rows, Hkv, dh)")
     rows, H, dh = q.shape
-    Hkv = k.shape[1]
-    _need(k.shape[0] == rows and k.shape[2] == dh and Hkv > 0 and H % Hkv == 0, who, "k and v must have q's rows and head size, and heads that divide q's")
-    _need(seq_off.dim() == 1 and seq_off.shape[0] >= 1, who, "seq_off (B + 1,)")
+    n, Hkv, e = k.shape
+    if n != rows or e != dh or Hkv < 1 or H % Hkv:
+        _refuse(who, "k and v must have q's rows and head size, and heads that divide q's")
+    if seq_off.dim() != 1 or seq_off.shape[0] < 1:
+        _refuse(who, "seq_off must be (B + 1,)")
     B = seq_off.shape[0] - 1
     dt = _operands(who, q, k, v)
-    seq_off, text_len = _index(who, "seq_off", seq_off, B + 1, q), _index(who, "text_len", text_len, B, q)
+    off, keep1 = _index(who, "seq_off", seq_off, B + 1, q)
+    text, keep2 = _index(who, "text_len", text_len, B, q)
     o = _out(who, out, q)
-    st, guard = _launch_on(q)
     q, k, v = _heads(q), _heads(k), _heads(v)
-    with guard:
-        _lib.check(_lib.load().vle_op_window_attention(
-            st, dt, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-            o.data_ptr(), seq_off.data_ptr(), _p(text_len), rows, B, H, Hkv, dh, int(window), int(sinks),
-            1.0 / math.sqrt(dh) if scale is None else float(scale), int(out is None)))
+    (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
+    _call(q, "vle_op_window_attention", dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, o.data_ptr(), off, text, rows, B, H, Hkv,
+          dh, window, sinks, dh ** -0.5 if scale is None else scale, out is None)
     return o
 
 
@@ -488,20 +503,21 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     seq_off[b] .. seq_off[b + 1] - 1; None: one row each) becomes key start[b] + r - seq_off[b]; mass (n_pages, Hkv, page_size) fp32 becomes 0 there.
     Rows of no sequence, positions past the table and page ids outside the pool are dropped; two rows must not go to one slot."""
     who = "paged_kv_write"
-    _need(k.dim() == 3 and v.shape == k.shape, who, "k and v must have one shape (rows, heads, dh)")
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
-    _need(k.shape[1] == Hkv and k.shape[2] == dh, who, f"k and v must have the pages' heads and head size ({Hkv}, {dh})")
-    _need(k_pages.data_ptr() != v_pages.data_ptr() or k_pages.numel() == 0, who, "keys and values need pages of their own")
-    rows = k.shape[0]
-    _need(seq_off is not None or rows == B, who, "without seq_off there is one row per sequence")
+    rows = k.shape[0] if k.dim() == 3 else 0
+    if k.shape != (rows, Hkv, dh) or v.shape != k.shape:
+        _refuse(who, f"k and v must be (rows, {Hkv}, {dh}), the pages' heads and head size")
+    if k_pages.data_ptr() == v_pages.data_ptr() and k_pages.numel():
+        _refuse(who, "keys and values need pages of their own")
+    if seq_off is None and rows != B:
+        _refuse(who, "without seq_off there is one row per sequence")
     dt = _operands(who, k, v, k_pages, v_pages)
-    start, seq_off = _index(who, "start", start, B, k), _index(who, "seq_off", seq_off, B + 1, k)
-    st, guard = _launch_on(k)
+    at, keep1 = _index(who, "start", start, B, k)
+    off, keep2 = _index(who, "seq_off", seq_off, B + 1, k)
     k, v = _heads(k), _heads(v)
-    with guard:
-        _lib.check(_lib.load().vle_op_paged_kv_write(
-            st, dt, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), _p(mass),
-            page_table.data_ptr(), start.data_ptr(), _p(seq_off), rows, B, Hkv, dh, n_pages, W, ps))
+    (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
+    _call(k, "vle_op_paged_kv_write", dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, k_pages.data_ptr(), v_pages.data_ptr(),
+          None if mass is None else mass.data_ptr(), page_table.data_ptr(), at, off, rows, B, Hkv, dh, n_pages, W, ps)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -523,23 +539,21 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     what kv_evict goes by.  Sequences may share pages (their weights are then added in no fixed order).  The split follows the width of
     page_table: hand a table as wide as the longest sequence needs."""
     who = "paged_decode_attention"
-    _need(q.dim() == 3, who, "q (B, H, dh)")
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
-    H = q.shape[1]
-    _need(q.shape[0] == B and q.shape[2] == dh and Hkv > 0 and H % Hkv == 0, who, "q must have the table's sequences, the pages' head size and a multiple of their heads")
+    H = q.shape[1] if q.dim() == 3 else 0
+    if q.shape != (B, H, dh) or Hkv < 1 or H < 1 or H % Hkv:
+        _refuse(who, "q must be (B, H, dh): the table's sequences, the pages' head size, a multiple of their heads")
     dt = _operands(who, q, k_pages, v_pages)
-    lengths, text_len = _index(who, "lengths", lengths, B, q), _index(who, "text_len", text_len, B, q)
-    window, sinks = int(window), int(sinks)
+    n, keep1 = _index(who, "lengths", lengths, B, q)
+    text, keep2 = _index(who, "text_len", text_len, B, q)
     o = _out(who, out, q)
-    st, guard = _launch_on(q)
     q = _heads(q)
-    n = _paged_decode_workspace(B, H, Hkv, dh, W, ps, window, sinks, text_len is not None, mass is not None)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None  # per call: two calls, or two graphs, share none
-    with guard:
-        _lib.check(_lib.load().vle_op_paged_decode_attention(
-            st, dt, q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-            _p(text_len), _p(mass), _p(ws), n, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
-            1.0 / math.sqrt(dh) if scale is None else float(scale)))
+    qr, qh, _ = q.stride()
+    room = _paged_decode_workspace(dt, B, H, Hkv, dh, W, ps, window, sinks, text is not None, mass is not None)
+    ws = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None  # per call: two calls, or two graphs, share none
+    _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), n, text,
+          None if mass is None else mass.data_ptr(), ws.data_ptr() if room else None, room, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
+          dh ** -0.5 if scale is None else scale)
     return o
 
 
@@ -553,18 +567,18 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     positions, ascending, -1 past the end; lengths int32 (B,) = min(lengths, budget)): the pages behind the new lengths are free.
     A page must belong to one sequence alone here."""
     who = "kv_evict"
+    if mass is None:
+        _refuse(who, "mass is needed")
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
-    _need(mass is not None, who, "mass is needed")
-    _need(k_pages.data_ptr() != v_pages.data_ptr() or k_pages.numel() == 0, who, "keys and values need pages of their own")
-    budget = int(budget)
-    _need(budget >= 1, who, "budget must be 1 at least")
+    if k_pages.data_ptr() == v_pages.data_ptr() and k_pages.numel():
+        _refuse(who, "keys and values need pages of their own")
+    if budget < 1:
+        _refuse(who, "budget must be 1 at least")
     dt = _operands(who, k_pages, v_pages)
-    lengths, text_len = _index(who, "lengths", lengths, B, k_pages), _index(who, "text_len", text_len, B, k_pages)
-    st, guard = _launch_on(k_pages)
-    kept = torch.empty(B, Hkv, budget, dtype=torch.int32, device=k_pages.device)
-    left = torch.empty(B, dtype=torch.int32, device=k_pages.device)
-    with guard:
-        _lib.check(_lib.load().vle_op_kv_evict(
-            st, dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _p(text_len), kept.data_ptr(),
-            left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget, int(recent), int(sinks)))
+    n, keep1 = _index(who, "lengths", lengths, B, k_pages)
+    text, keep2 = _index(who, "text_len", text_len, B, k_pages)
+    kept = page_table.new_empty((B, Hkv, budget))
+    left = page_table.new_empty((B,))
+    _call(k_pages, "vle_op_kv_evict", dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), n, text, kept.data_ptr(),
+          left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget, recent, sinks)
     return kept, left
