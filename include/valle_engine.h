@@ -377,7 +377,7 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  * (valle/models/valle.py:1019-1033) is the case window = 0 of the first.
  *   row i of a sequence sees key j  iff  j < text_len  or  (j <= i and (window == 0 or i - j < window or j < sinks))
  * dtype VLE_DTYPE_F32 / _BF16 (T); head size a multiple of 8, <= 128; nhead a multiple of nhead_kv (query head h reads key-value head
- * h / (nhead / nhead_kv)), at most 256 per key-value head; strides in elements, every row and head on 16 bytes; scale > 0
+ * h / (nhead / nhead_kv)), at most 256 per key-value head; strides in elements, every row and head on 16 bytes, rows less than 2^24 elements apart; scale > 0
  * (1 / sqrt(dh) as a rule).  All pointers DEVICE, index arrays int32.  A bad argument is refused with VLE_EINVAL before any launch;
  * what index arrays hold is bounded inside the kernels: offsets and lengths are clamped to the rows / the table, and a page id outside
  * [0, n_pages) is never followed -- its keys are absent.  The HIP device current at the call must be the stream's.

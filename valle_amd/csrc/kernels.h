@@ -520,6 +520,7 @@ struct PagedDecodeArgs {
 };
 struct PagedDecodePlan {  // split of the cache's length, and the workspace it needs
   int tiles, nsplit, nw, score_lds;  // score_lds > 0: scores of a head kept in LDS
+  bool stream;                       // more keys and values than the memory-side cache holds: read past it
   size_t ml_floats, o_floats, score_floats;
 };
 PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int W, int ps, int window, int sinks, bool text, bool mass);

@@ -284,9 +284,9 @@ extern "C" int vle_op_linear_fp8(void* stream, const void* a8, const float* a_sc
 
 // ---- attention with a window, and the paged key-value cache ----------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-static bool vec_strides(int dtype, int64_t row, int64_t head) {  // every row and head starts on 16 bytes
+static bool vec_strides(int dtype, int64_t row, int64_t head) {  // every row and head starts on 16 bytes, offsets inside a tile fit 32 bits
   const int64_t v = dtype == DT_F32 ? 4 : 8;
-  return row >= 0 && head >= 0 && row % v == 0 && head % v == 0;
+  return row >= 0 && head >= 0 && row % v == 0 && head % v == 0 && row < (1 << 24);
 }
 static const char* heads_fault(int dtype, int32_t nhead, int32_t nhead_kv, int32_t dh) {
   if (dtype != DT_F32 && dtype != DT_BF16) return "dtype must be f32 or bf16";
@@ -324,7 +324,7 @@ extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, i
   if (!q || !k || !v || !out || !seq_off_dev) return op_refuse(op, "null operand");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !vec_strides(dtype, q_row, q_head) ||
       !vec_strides(dtype, k_row, k_head) || !vec_strides(dtype, v_row, v_head))
-    return op_refuse(op, "rows and heads must start on 16 bytes");
+    return op_refuse(op, "rows and heads must start on 16 bytes, rows less than 2^24 elements apart");
   WindowAttnArgs a;
   a.q = q; a.k = k; a.v = v; a.out = out;
   a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
@@ -348,7 +348,7 @@ extern "C" int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int
   if (!k || !v || !k_pages || !v_pages || !page_table_dev || !start_dev) return op_refuse(op, "null operand");
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || !vec_strides(dtype, k_row, k_head) ||
       !vec_strides(dtype, v_row, v_head))
-    return op_refuse(op, "rows and heads must start on 16 bytes");
+    return op_refuse(op, "rows and heads must start on 16 bytes, rows less than 2^24 elements apart");
   PagedWriteArgs a;
   a.k = k; a.v = v; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
   a.k_pages = k_pages; a.v_pages = v_pages; a.mass = mass; a.table = page_table_dev; a.start = start_dev; a.seq_off = seq_off_dev;
@@ -380,7 +380,7 @@ extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void
   if (B == 0) return VLE_OK;
   if (!q || !k_pages || !v_pages || !page_table_dev || !lengths_dev || !out) return op_refuse(op, "null operand");
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || !vec_strides(dtype, q_row, q_head))
-    return op_refuse(op, "rows and heads must start on 16 bytes");
+    return op_refuse(op, "rows and heads must start on 16 bytes, rows less than 2^24 elements apart");
   const PagedDecodePlan p = paged_decode_plan(dtype, B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, text_len_dev != nullptr, mass != nullptr);
   const int64_t need = (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need)) return op_refuse(op, "workspace too small (vle_op_paged_decode_workspace_bytes)");

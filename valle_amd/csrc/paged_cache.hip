@@ -109,23 +109,29 @@ int launch_paged_write(hipStream_t st, int dtype, const PagedWriteArgs& a) {
 // lane (g, c) loads dims c * DPL .. + DPL - 1 of its group's 8 keys (four whole rows per instruction) and one byte-permute per packed pair turns
 // them into the operands of DPL products, product j giving dims 4-lane-slot * DPL + j.  No LDS, no barrier in the loop; a group of one
 // head leaves 15 columns empty, which the matrix pipe has room for (it needs 1/16 of the time the HBM takes for the same keys).
-template <int N>
+// NT: past the memory-side cache
+template <bool NT, typename V>
+__device__ inline V pd_load(const void* p) {
+  if constexpr (NT) return __builtin_nontemporal_load((const V*)p);
+  else return *(const V*)p;
+}
+template <bool NT, int N>
 __device__ inline void pd_load_words(unsigned (&dst)[N], const void* src) {  // N = 2, 4 or 8 words of 32 bits, from 8 or 16 aligned bytes on
   if constexpr (N == 2) {
-    const pc_u32x2 x = *reinterpret_cast<const pc_u32x2*>(src);
+    const pc_u32x2 x = pd_load<NT, pc_u32x2>(src);
     dst[0] = x[0];
     dst[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const pc_u32x4 x = reinterpret_cast<const pc_u32x4*>(src)[i];
+      const pc_u32x4 x = pd_load<NT, pc_u32x4>((const pc_u32x4*)src + i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) dst[4 * i + j] = x[j];
     }
   }
 }
 
-template <typename T, int DHT, int NW, bool WHOLE>  // WHOLE: dh == DHT, no lane is ever outside the head
+template <typename T, int DHT, int NW, bool WHOLE, bool NT>  // WHOLE: dh == DHT, no lane is ever outside the head
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(PagedDecodeArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int TK = pc_tile<T>(), ST = TK / 16;  // 16-key score tiles of a step
@@ -199,7 +205,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
 #pragma unroll
         for (int i = 0; i < KV; ++i) {
           if (!WHOLE) kf[st][i] = pc_u32x4{0u, 0u, 0u, 0u};
-          if (WHOLE || i * 4 * KE + g * KE < dh) kf[st][i] = *reinterpret_cast<const pc_u32x4*>(kbase + at + koff + i * 4 * KE);
+          if (WHOLE || i * 4 * KE + g * KE < dh) kf[st][i] = pd_load<NT, pc_u32x4>(kbase + at + koff + i * 4 * KE);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -207,7 +213,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
 #pragma unroll
             for (int i = 0; i < VW; ++i) vf[4 * st + r][i] = 0;
           }
-          if (vin) pd_load_words(vf[4 * st + r], vbase + at + voff + r * dh);
+          if (vin) pd_load_words<NT>(vf[4 * st + r], vbase + at + voff + r * dh);
         }
       }
     } else {
@@ -226,7 +232,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
           for (int i = 0; i < VW; ++i) vf[4 * st + r][i] = 0;
-          if ((page[st] >= 0) & vin & sp.sees(k4 + r)) pd_load_words(vf[4 * st + r], pv + r * dh);  // what nobody sees may hold anything, NaN included
+          if ((page[st] >= 0) & vin & sp.sees(k4 + r)) pd_load_words<false>(vf[4 * st + r], pv + r * dh);  // what nobody sees may hold anything, NaN included
         }
       }
     }
@@ -442,12 +448,16 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
   const int tk = dtype == DT_F32 ? 16 : 32, ng = std::min(16, G);
   p.tiles = std::max(1, pd_tiles_bound(W, ps, window, sinks, text, tk));
   const int64_t groups = (int64_t)B * Hkv * ((G + 15) / 16), H = (int64_t)Hkv * G;
+  // Workgroups of 4 waves that are resident at once: 256 CUs, 3 each (5 at head size 64).  One round of equal parts: 32 splits of three 40k - 60k
+  // caches with 8 heads take 113 us, 43 (one third more than fit) 128, 64 (two rounds) 116, 128 (shorter parts, a longer join) 121.
+  const int64_t slots = 256 * (dh <= 64 ? 5 : 3);
   p.nsplit = 1;
   p.nw = groups < 512 && ng <= 8 ? 8 : 4;  // 8 waves: their outputs fit 32 KB of LDS for up to 8 heads
   if (groups < 512 && p.tiles > 8 * p.nw) {
     p.nw = 4;
-    p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), (3072 + groups - 1) / groups);
+    p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), std::max((int64_t)1, slots / groups));
   }
+  p.stream = (int64_t)p.tiles * tk * B * Hkv * dh * (dtype == DT_F32 ? 8 : 4) > (int64_t)128 << 20;
   // weights: by the workgroup that has all of a head's scores, where they fit beside its outputs; else by the join
   p.score_lds = mass && p.nsplit == 1 && G <= 16 && (int64_t)p.tiles * tk * ng <= 7168 ? p.tiles * tk : 0;
   const bool join_mass = mass && p.score_lds == 0;
@@ -462,8 +472,9 @@ static void pd_launch_nw(hipStream_t st, const PagedDecodePlan& p, const PagedDe
   const int ng = std::min(16, a.G);
   const size_t lds = ((size_t)NW * ng * DHT + NW * 32 + 32 + (size_t)ng * p.score_lds) * sizeof(float);
   const dim3 grid(p.nsplit, a.Hkv * a.GT, B), block(NW * 64);
-  if (a.dh == DHT) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, false>), grid, block, lds, st, a);
+  if (a.dh != DHT) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, false, false>), grid, block, lds, st, a);
+  else if (p.stream) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, true>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, false>), grid, block, lds, st, a);
 }
 
 template <typename T, int DHT>
@@ -657,8 +668,10 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
 // The keys that stay move up in place: row i takes the place of kept[i] >= i.  Rows move in ascending chunks, all of a head's columns of one pool
 // (or a slice of them) by ONE workgroup: a chunk's targets lie below every later chunk's sources, so the next chunk may be on its way while this
 // one is stored, and only the rows of one chunk can overwrite each other's sources -- a barrier between its loads' return and its stores rules
-// that out.  HBM-bound; two chunks of 8 vectors per thread in flight.
-constexpr int MV_T = 256, MV_U = 8, MV_TAB = 4096;
+// that out.  HBM-bound: two chunks of 32 KB in flight per workgroup.  1024 threads of 2 vectors a chunk: 32 sequences of 4.5k - 9k keys, 8 heads of 128,
+// back to 4096, together with the selection 268 us (1.09 GB, 4.1 TB/s; a plain copy reaches 4.9 here); 256 threads of 8 vectors, whose chunk takes as
+// many bytes but whose lanes walk it alone: 302.
+constexpr int MV_T = 1024, MV_U = 2, MV_TAB = 4096;
 
 template <typename V>
 __device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* kept, const int32_t* tab, const int32_t* sh_tab, int h, int vpr, int e0,
@@ -676,27 +689,27 @@ __device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* ke
       from[u] = mine && row < n ? kept[row] : -1;
     }
   };
-  // loads are unconditional (from the pool's first vector where there is nothing to move), so that the waits for them can be counted
-  auto load_rows = [&](int base, V (&x)[MV_U], V* (&dst)[MV_U]) {
+  auto place = [&](int page, int j) { return pool + (int64_t)page * page_vecs + (int64_t)(h * ps + (j & (ps - 1))) * vpr + e; };
+  // loads are unconditional (from the pool's first vector where there is nothing to move), so that the waits for them can be counted;
+  // bit u of the result: vector u is to be stored
+  auto load_rows = [&](int base, V (&x)[MV_U]) -> unsigned {
+    unsigned moves = 0;
 #pragma unroll
     for (int u = 0; u < MV_U; ++u) {
       const int row = base + u * rows + row0;
-      const V* src = pool;
-      dst[u] = nullptr;
-      if (from[u] > row && from[u] < len) {
-        const int sp = page_of(from[u]), dp = page_of(row);
-        if ((unsigned)sp < (unsigned)a.n_pages && (unsigned)dp < (unsigned)a.n_pages) {
-          src = pool + (int64_t)sp * page_vecs + (int64_t)(h * ps + (from[u] & (ps - 1))) * vpr + e;
-          dst[u] = pool + (int64_t)dp * page_vecs + (int64_t)(h * ps + (row & (ps - 1))) * vpr + e;
-        }
-      }
-      x[u] = *src;
+      const bool go = (from[u] > row) & (from[u] < len);
+      const int sp = go ? page_of(from[u]) : -1, dp = go ? page_of(row) : -1;
+      const bool there = ((unsigned)sp < (unsigned)a.n_pages) & ((unsigned)dp < (unsigned)a.n_pages);
+      x[u] = *(there ? place(sp, from[u]) : pool);
+      moves |= there ? 1u << u : 0u;
     }
+    return moves;
   };
   const int step = MV_U * rows;
-  auto turn = [&](int base, V (&x)[MV_U], V* (&dst)[MV_U], V (&x2)[MV_U], V* (&dst2)[MV_U]) {
+  auto turn = [&](int base, V (&x)[MV_U], unsigned moves, V (&next)[MV_U]) -> unsigned {
+    unsigned m2 = 0;
     if (base + step < n) {
-      load_rows(base + step, x2, dst2);
+      m2 = load_rows(base + step, next);
       load_kept(base + 2 * step);
     }
 #pragma unroll
@@ -704,23 +717,26 @@ __device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* ke
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < MV_U; ++u)
-      if (dst[u] != nullptr) *dst[u] = x[u];
+      if (moves >> u & 1) {
+        const int row = base + u * rows + row0;
+        *place(page_of(row), row) = x[u];
+      }
+    return m2;
   };
   V x[MV_U], y[MV_U];
-  V *dx[MV_U], *dy[MV_U];
   load_kept(0);
-  load_rows(0, x, dx);
+  unsigned mx = load_rows(0, x), my;
   load_kept(step);
   for (int base = 0; base < n; base += 2 * step) {
-    turn(base, x, dx, y, dy);
-    if (base + step < n) turn(base + step, y, dy, x, dx);
+    my = turn(base, x, mx, y);
+    if (base + step < n) mx = turn(base + step, y, my, x);
   }
 }
 
-// blockIdx.z: 2 * slices parts of the keys and values, then the weights
+// blockIdx.z: the weights, then 2 * slices parts of the keys and values
 __global__ __launch_bounds__(MV_T) void kv_evict_move_kernel(EvictArgs a, int vpr, int slices) {
   __shared__ int32_t sh_tab[MV_TAB];
-  const int h = blockIdx.x, b = blockIdx.y, what = blockIdx.z;
+  const int h = blockIdx.x, b = blockIdx.y, what = (int)blockIdx.z - 1;
   const EvictRow r = evict_row(a, b);
   if (r.n <= a.budget) return;
   const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
@@ -730,7 +746,7 @@ __global__ __launch_bounds__(MV_T) void kv_evict_move_kernel(EvictArgs a, int vp
   if (cached != nullptr)
     for (int i = threadIdx.x; i < used; i += MV_T) sh_tab[i] = tab[i];
   __syncthreads();
-  if (what == 2 * slices) {
+  if (what < 0) {
     evict_move<float>(a.mass, a, kept, tab, cached, h, 1, 0, 1, r.n);
   } else {
     const int width = vpr / slices;
@@ -746,7 +762,10 @@ int launch_kv_evict(hipStream_t st, int dtype, const EvictArgs& a, int B, int dh
   else if (most <= 16 * EV_T) hipLaunchKernelGGL((kv_evict_select_kernel<16>), sgrid, dim3(EV_T), 0, st, a);
   else hipLaunchKernelGGL((kv_evict_select_kernel<0>), sgrid, dim3(EV_T), 0, st, a);
   const int vpr = dh * (dtype == DT_F32 ? 4 : 2) / 16;
-  const int slices = vpr % 8 == 0 ? vpr / 8 : 1;  // whole 128-byte lines of a row each
+  // Slices of whole 128-byte lines; of 64 bytes where that leaves fewer than two workgroups a CU (measured with 256 threads: 4 sequences of 16 heads
+  // of 64: 40 -> 33 us; with 32 sequences of 8 heads of 128 half lines cost 295 -> 331 us)
+  int slices = vpr % 8 == 0 ? vpr / 8 : 1;
+  if (vpr % 4 == 0 && (int64_t)B * a.Hkv * 2 * slices < 512) slices = vpr / 4;
   hipLaunchKernelGGL(kv_evict_move_kernel, dim3(a.Hkv, B, 2 * slices + 1), dim3(MV_T), 0, st, a, vpr, slices);
   return 0;
 }

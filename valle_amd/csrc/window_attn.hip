@@ -180,25 +180,44 @@ __device__ constexpr int wa_key(int row) {
   return NV % 16 == 0 ? (row & 15) : NV % 8 == 0 ? (row & 7) : ((row >> 1) & 3);
 }
 
-__device__ inline void wa_dma(const void* src, unsigned char* dst) {  // 16 bytes per lane to dst + 16 * lane (dst wave-uniform)
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// 16 bytes per lane from base + off to LDS address dst + 16 * lane (base and dst wave-uniform).  Not the builtin: the compiler takes any later LDS
+// read it cannot tell apart -- the transposing ones -- for a reader of what is in flight and waits for all of it, so that no tile is ever fetched ahead.
+// The waits for these loads are the kernels' own, ahead of the barrier that hands a tile over.
+__device__ inline void wa_dma(const void* base, unsigned off, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
 
-// One tile of TK rows (NV vectors of VE elements each) of K or V into LDS, by the whole workgroup.  Rows past the sequence repeat its last one
-// and vectors past the head its first one: what they hold is never visible.
+// Stages tiles of TK rows (NV 16-byte vectors each) of K or V into LDS, by the whole workgroup.  Rows past the sequence repeat its last one and
+// vectors past the head its first one: what they hold is never visible.  A lane's place in a tile is worked out once; a tile inside the sequence
+// then costs scalar arithmetic alone.  (Byte offsets inside a tile are 32-bit: row strides are below 2^24 elements, checked at the entry.)
 template <typename T, int TK, int NV>
-__device__ inline void stage_tile(const T* base, int64_t row_stride, int kt0, int len, int dh, unsigned char* dst, int w_uniform) {
-  constexpr int VE = 16 / (int)sizeof(T);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+struct Stager {
+  static constexpr int VE = 16 / (int)sizeof(T), N = TK * NV / 256;
+  const T* base;
+  unsigned stride;  // bytes
+  int len, wu;
+  unsigned off[N];
+  __device__ Stager(const T* b, int64_t row_stride, int l, int dh, int w_uniform) : base(b), stride((unsigned)row_stride * sizeof(T)), len(l), wu(w_uniform) {
 #pragma unroll
-  for (int i = 0; i < TK * NV / 256; ++i) {
-    const int idx = (i * 4 + w) * 64 + lane;
-    const int row = idx / NV, slot = idx % NV;
-    int vec = slot ^ wa_key<NV>(row);
-    if (vec * VE >= dh) vec = 0;
-    wa_dma(base + (int64_t)min(kt0 + row, len - 1) * row_stride + vec * VE, dst + (i * 4 + w_uniform) * 1024);
+    for (int i = 0; i < N; ++i) off[i] = row(i) * stride + vec(i, dh) * 16;
   }
-}
+  __device__ int row(int i) const { return ((i * 4 + wu) * 64 + (int)(threadIdx.x & 63)) / NV; }
+  __device__ int vec(int i, int dh) const {
+    const int v = (((i * 4 + wu) * 64 + (int)(threadIdx.x & 63)) % NV) ^ wa_key<NV>(row(i));
+    return v * VE < dh ? v : 0;
+  }
+  __device__ void operator()(int kt0, int dh, const unsigned char* dst) const {
+    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)dst) + wu * 1024;
+    const char* src = (const char*)base + (int64_t)kt0 * stride;
+    if (kt0 + TK <= len) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) wa_dma(src, off[i], to + i * 4096);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) wa_dma(src, min(row(i), len - 1 - kt0) * stride + vec(i, dh) * 16, to + i * 4096);
+    }
+  }
+};
 
 }  // namespace
 
@@ -239,15 +258,16 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
       wa_u32x4 x = {0u, 0u, 0u, 0u};
       if (ks * 32 + g * 8 < dh) x = *reinterpret_cast<const wa_u32x4*>(qp + ks * 32 + g * 8);
       qf[f][ks] = __builtin_bit_cast(wa_bf16x8, x);
+      asm volatile("" : "+v"(qf[f][ks]));  // waited for here, once: a wait at the first use would stand inside the loop and take the tiles in flight with it
     }
   }
 
-  const float sl2 = a.sl2, defer = WA_DEFER / a.sl2;
-  float m[QW];  // running maximum of the raw scores of the row, shared by its 4 lanes
+  const float sl2 = a.sl2;
+  float M[QW];  // reference of the row's scores, shared by its 4 lanes: their maximum when it was last moved; -inf: no key yet
   wa_f32x4 ol[QW], o[QW][EB];
 #pragma unroll
   for (int f = 0; f < QW; ++f) {
-    m[f] = -INFINITY;
+    M[f] = -INFINITY;
     ol[f] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int eb = 0; eb < EB; ++eb) o[f][eb] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -255,8 +275,9 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
   const wa_bf16x8 ones = __builtin_bit_cast(wa_bf16x8, wa_s16x8{0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80});
   auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
 
-  stage_tile<bf16_t, TK, NV>(kb, a.k_row, key0(0), len, dh, smem, wu);
-  stage_tile<bf16_t, TK, NV>(vb, a.v_row, key0(0), len, dh, smem + HALF, wu);
+  const Stager<bf16_t, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
+  stage_k(key0(0), dh, smem);
+  stage_v(key0(0), dh, smem + HALF);
   for (int t = 0; t < ti.tt; ++t) {
     const int kt0 = key0(t);
     const unsigned char* Ks = smem + (t & 1) * BUF;
@@ -265,8 +286,8 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
     __syncthreads();                                  // everyone's have; everyone is done with tile t - 1
     if (t + 1 < ti.tt) {
       unsigned char* nb = smem + ((t + 1) & 1) * BUF;
-      stage_tile<bf16_t, TK, NV>(kb, a.k_row, key0(t + 1), len, dh, nb, wu);
-      stage_tile<bf16_t, TK, NV>(vb, a.v_row, key0(t + 1), len, dh, nb + HALF, wu);
+      stage_k(key0(t + 1), dh, nb);
+      stage_v(key0(t + 1), dh, nb + HALF);
     }
     bool some = false, all = true;
 #pragma unroll
@@ -275,96 +296,119 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
       all &= see[f].all(kt0, TK);
     }
     if (!__any(some)) continue;
-    const bool unmasked = __all(all);
+    const bool unmasked = __all(all);  // a masked tile's key that is not finite makes the row NaN: computed again at the end
 
-    // ---- S^T = K Q^T ----
+    // ---- S^T = K Q^T: the accumulators start from the mask (0 or -inf) ----
     wa_f32x4 s[QW][4];
+    auto scores = [&]() {
+      wa_bf16x8 ka[2][KS];  // the next 16 keys' fragments are read while these are multiplied
+      auto read_k = [&](wa_bf16x8 (&d)[KS], int kb4) {
 #pragma unroll
-    for (int kb4 = 0; kb4 < 4; ++kb4) {
+        for (int ks = 0; ks < KS; ++ks)
+          d[ks] = *reinterpret_cast<const wa_bf16x8*>(Ks + (kb4 * 16 + c) * ROW + (((ks * 4 + g) ^ wa_key<NV>(c)) << 4));
+      };
+      read_k(ka[0], 0);
 #pragma unroll
-      for (int f = 0; f < QW; ++f) s[f][kb4] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kb4 = 0; kb4 < 4; ++kb4) {
+        if (kb4 < 3) read_k(ka[(kb4 + 1) & 1], kb4 + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const wa_bf16x8 ka = *reinterpret_cast<const wa_bf16x8*>(Ks + (kb4 * 16 + c) * ROW + (((ks * 4 + g) ^ wa_key<NV>(c)) << 4));
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int f = 0; f < QW; ++f) s[f][kb4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[f][ks], s[f][kb4], 0, 0, 0);
+          for (int f = 0; f < QW; ++f) s[f][kb4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[kb4 & 1][ks], qf[f][ks], s[f][kb4], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    // ---- online softmax ----
-    wa_bf16x8 pf[QW][2];
+    };
+    if (unmasked) {
 #pragma unroll
-    for (int f = 0; f < QW; ++f) {
-      if (!unmasked) {
-        // tiles behind the head hold no key below hd, and as a rule only one edge of the window: one compare with a constant per score
-        const int hi = see[f].i - kt0 - g * 4, lo = see[f].lo - kt0 - g * 4;  // key number 16 kb4 + r of this lane is visible from lo to hi
-        if (t < ti.th) {
-          const int hd = see[f].hd - kt0 - g * 4;  // or below hd
+      for (int f = 0; f < QW; ++f)
+#pragma unroll
+        for (int kb4 = 0; kb4 < 4; ++kb4) s[f][kb4] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+      scores();
+    } else {
+#pragma unroll
+      for (int f = 0; f < QW; ++f) {
+        // key number 16 kb4 + r of this lane is visible from lo to hi, or, in a tile of the head, below hd: compares with constants, as few as the tile needs
+        const int hi = see[f].i - kt0 - g * 4, lo = see[f].lo - kt0 - g * 4, hd = see[f].hd - kt0 - g * 4;
+        auto mask = [&](auto hidden) {
 #pragma unroll
           for (int kb4 = 0; kb4 < 4; ++kb4)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              s[f][kb4][r] = (kb4 * 16 + r >= hd) & ((kb4 * 16 + r < lo) | (kb4 * 16 + r > hi)) ? -INFINITY : s[f][kb4][r];
-        } else {
-          if (__any(see[f].i < kt0 + TK - 1)) {
-#pragma unroll
-            for (int kb4 = 0; kb4 < 4; ++kb4)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                s[f][kb4][r] = kb4 * 16 + r > hi ? -INFINITY : s[f][kb4][r];
-          }
-          if (__any(see[f].lo > kt0)) {
-#pragma unroll
-            for (int kb4 = 0; kb4 < 4; ++kb4)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                s[f][kb4][r] = kb4 * 16 + r < lo ? -INFINITY : s[f][kb4][r];
-          }
-        }
+            for (int r = 0; r < 4; ++r) s[f][kb4][r] = hidden(kb4 * 16 + r) ? -INFINITY : 0.f;
+        };
+        if (t < ti.th) mask([=](int k) { return (k >= hd) & ((k < lo) | (k > hi)); });
+        else if (!__any(lo > -g * 4)) mask([=](int k) { return k > hi; });
+        else if (!__any(hi < TK - 1 - g * 4)) mask([=](int k) { return k < lo; });
+        else mask([=](int k) { return (k < lo) | (k > hi); });
       }
+      scores();
+    }
+    // ---- online softmax: scores relative to the row's reference M, both in units of the exp2 argument ----
+    wa_bf16x8 pf[QW][2];
+#pragma unroll
+    for (int f = 0; f < QW; ++f) {
+      // s sl2 - M in one fma: what the rounding of M leaves is a factor of the whole row and cancels, up to scores of 2^31, where it passes the
+      // exponent's range and the row is computed again
+      const float nm = M[f] == -INFINITY ? 0.f : -M[f];
+#pragma unroll
+      for (int kb4 = 0; kb4 < 4; ++kb4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[f][kb4][r] = fmaf(s[f][kb4][r], sl2, nm);
       float mt = fmaxf(fmaxf(s[f][0][0], s[f][0][1]), fmaxf(s[f][0][2], s[f][0][3]));
 #pragma unroll
       for (int kb4 = 1; kb4 < 4; ++kb4) mt = fmaxf(mt, fmaxf(fmaxf(s[f][kb4][0], s[f][kb4][1]), fmaxf(s[f][kb4][2], s[f][kb4][3])));
-      // the reference stays while no score exceeds it by more than `defer`: the result does not depend on it, O and the sum carry the same factor
-      if (!__all(mt <= m[f] + defer)) {
-        const float mn = fmaxf(m[f], rows4_max(mt));
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f((m[f] - ref) * sl2);
-        m[f] = mn;
+      // the reference stays while no score exceeds it by more than WA_DEFER: the result does not depend on it, O and the sum carry the same factor
+      if (!__all((mt <= WA_DEFER) & (M[f] != -INFINITY))) {
+        mt = rows4_max(mt);
+        const bool begun = M[f] != -INFINITY;
+        const float d = begun ? fmaxf(mt, 0.f) : (mt == -INFINITY ? 0.f : mt);
+        const float alpha = begun ? __builtin_amdgcn_exp2f(-d) : 1.f;
+        M[f] = begun ? M[f] + d : mt;
+#pragma unroll
+        for (int kb4 = 0; kb4 < 4; ++kb4) s[f][kb4] -= d;
         ol[f] *= alpha;
 #pragma unroll
         for (int eb = 0; eb < EB; ++eb) o[f][eb] *= alpha;
       }
-      // s sl2 - m sl2 in one fma: what the rounding of m sl2 leaves is a factor of the whole row and cancels, up to scores of 2^31, where it
-      // passes the exponent's range and the row is computed again
-      const float nm = m[f] == -INFINITY ? 0.f : -m[f] * sl2;
 #pragma unroll
       for (int kb4 = 0; kb4 < 4; ++kb4)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[f][kb4][r] = __builtin_amdgcn_exp2f(fmaf(s[f][kb4][r], sl2, nm));
+        for (int r = 0; r < 4; ++r) s[f][kb4][r] = __builtin_amdgcn_exp2f(s[f][kb4][r]);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int tt = 0; tt < 8; ++tt) pf[f][j][tt] = (__bf16)s[f][2 * j + (tt >> 2)][tt & 3];
     }
     // ---- O^T += V^T P^T ----
+    // the transposing read hands lane c the elements V[k0 .. k0 + 3][16 eb + c] of the rows whose addresses lanes c / 4 supply
+    wa_s16x4 vr[2][2][2];  // [buffer][j][half]: the next 16 columns' fragments are read while these are multiplied
+    auto read_v = [&](wa_s16x4 (&d)[2][2], int eb) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = j * 32 + g * 4 + (c >> 2);
+        const unsigned char* va = Vs + key * ROW + (((eb * 2 + ((c & 3) >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3);
+        d[j][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va));
+        d[j][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va + 16 * ROW));  // the swizzle has a period of 16 rows
+      }
+    };
+    read_v(vr[0], 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int f = 0; f < QW; ++f) ol[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[f][j], ol[f], 0, 0, 0);
 #pragma unroll
-    for (int eb = 0; eb < EB; ++eb)
+    for (int eb = 0; eb < EB; ++eb) {
+      if (eb + 1 < EB) read_v(vr[(eb + 1) & 1], eb + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        // the transposing read hands lane c the elements V[k0 .. k0 + 3][16 eb + c] of the rows whose addresses lanes c / 4 supply
-        const int key = j * 32 + g * 4 + (c >> 2);
-        const unsigned char* va = Vs + key * ROW + (((eb * 2 + ((c & 3) >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3);
-        const unsigned char* vh = va + 16 * ROW;  // the key of the swizzle has a period of 16 rows
-        const wa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va));
-        const wa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(vh));
+        const wa_s16x4 lo = vr[eb & 1][j][0], hi = vr[eb & 1][j][1];
         const wa_bf16x8 vf = __builtin_bit_cast(wa_bf16x8, wa_s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 #pragma unroll
         for (int f = 0; f < QW; ++f) o[f][eb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][j], o[f][eb], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 
 #pragma unroll
@@ -429,6 +473,7 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   for (int t = 0; t < KT; ++t) {
     qf[t] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
     if (t * 16 + g * 4 < dh) qf[t] = *reinterpret_cast<const wa_f32x4*>(qp + t * 16 + g * 4);
+    asm volatile("" : "+v"(qf[t]));  // as in the bf16 kernel
   }
   const float sl2 = a.sl2;
   float m = -INFINITY, l = 0.f;
@@ -437,8 +482,9 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   for (int j = 0; j < DPL; ++j) o[j] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
   auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
 
-  stage_tile<float, TK, NV>(kb, a.k_row, key0(0), len, dh, smem, wu);
-  stage_tile<float, TK, NV>(vb, a.v_row, key0(0), len, dh, smem + HALF, wu);
+  const Stager<float, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
+  stage_k(key0(0), dh, smem);
+  stage_v(key0(0), dh, smem + HALF);
   for (int t = 0; t < ti.tt; ++t) {
     const int kt0 = key0(t);
     const unsigned char* Ks = smem + (t & 1) * BUF;
@@ -447,8 +493,8 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
     __syncthreads();
     if (t + 1 < ti.tt) {
       unsigned char* nb = smem + ((t + 1) & 1) * BUF;
-      stage_tile<float, TK, NV>(kb, a.k_row, key0(t + 1), len, dh, nb, wu);
-      stage_tile<float, TK, NV>(vb, a.v_row, key0(t + 1), len, dh, nb + HALF, wu);
+      stage_k(key0(t + 1), dh, nb);
+      stage_v(key0(t + 1), dh, nb + HALF);
     }
     if (!__any(see.any(kt0, TK))) continue;
     wa_f32x4 s[2];

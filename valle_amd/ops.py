@@ -385,40 +385,34 @@ def _refuse(who: str, what: str):
 
 def _operands(who: str, first: torch.Tensor, *others: torch.Tensor) -> int:
     """One device, one type, no gradient asked for; -> the type's code."""
-    dt = _dt(first)
-    grad = first.requires_grad
-    where, what = first.device, first.dtype
+    what, where, grad = first.dtype, first.get_device(), first.requires_grad
     for t in others:
-        if t.dtype != what:
+        if t.dtype is not what:
             raise TypeError(f"{who}: dtypes {what} and {t.dtype} differ")
-        if t.device != where:
+        if t.get_device() != where:
             _refuse(who, "all tensors must be on one device")
         grad = grad or t.requires_grad
     if grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who} has no backward pass: detach its operands or call it under torch.no_grad()")
-    return dt
+    return _lib.DTYPE_BF16 if what is torch.bfloat16 else _dt(first)
 
 
-def _index(who: str, name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor):
-    """Address of an int32 vector of n values on like's device (None: NULL), and the tensor that must outlive the call."""
-    if t is None:
-        return None, None
-    if t.dtype != torch.int32:
+def _index(who: str, name: str, t: torch.Tensor, n: int, like: torch.Tensor) -> torch.Tensor:
+    """t, an int32 vector of n values on like's device, contiguous (the caller holds it until its launch)."""
+    if t.dtype is not torch.int32:
         raise TypeError(f"{who}: {name} must be int32, got {t.dtype}")
-    if t.shape != (n,):
+    if t.dim() != 1 or t.numel() != n:
         _refuse(who, f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         _refuse(who, f"{name} must be on {like.device}")
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t.data_ptr(), t
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t (rows, heads, dh) as it is where every row and head starts on 16 bytes, else a contiguous copy."""
-    v = 8 if t.dtype == torch.bfloat16 else 4
+    """t (rows, heads, dh) as it is where every row and head starts on 16 bytes and rows are not far apart, else a contiguous copy."""
+    m = 7 if t.dtype is torch.bfloat16 else 3
     r, h, e = t.stride()
-    if e == 1 and r % v == 0 and h % v == 0 and t.data_ptr() % 16 == 0:
+    if e == 1 and not (r | h) & m and r < 1 << 24 and not t.data_ptr() & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -433,19 +427,19 @@ def _out(who: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Ten
 
 def _pages(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, mass: Optional[torch.Tensor]):
     """Checks of a page pool; -> (n_pages, heads, page size, dh, sequences, table width)."""
-    shape, where = k_pages.shape, k_pages.device
+    shape, where = k_pages.shape, k_pages.get_device()
     if len(shape) != 4 or v_pages.shape != shape:
         _refuse(who, "k_pages and v_pages must have one shape (n_pages, heads, page_size, dh)")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         _refuse(who, "pages must be contiguous")
-    if page_table.dtype != torch.int32:
+    if page_table.dtype is not torch.int32:
         raise TypeError(f"{who}: page_table must be int32, got {page_table.dtype}")
-    if page_table.dim() != 2 or not page_table.is_contiguous() or page_table.device != where:
+    if page_table.dim() != 2 or not page_table.is_contiguous() or page_table.get_device() != where:
         _refuse(who, "page_table must be a contiguous (sequences, pages) tensor on the pages' device")
     if mass is not None:
-        if mass.dtype != torch.float32:
+        if mass.dtype is not torch.float32:
             raise TypeError(f"{who}: mass must be float32, got {mass.dtype}")
-        if mass.shape != shape[:3] or not mass.is_contiguous() or mass.device != where:
+        if mass.shape != shape[:3] or not mass.is_contiguous() or mass.get_device() != where:
             _refuse(who, "mass must be a contiguous (n_pages, heads, page_size) tensor on the pages' device")
     return (*shape, *page_table.shape)
 
@@ -484,12 +478,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
         _refuse(who, "seq_off must be (B + 1,)")
     B = seq_off.shape[0] - 1
     dt = _operands(who, q, k, v)
-    off, keep1 = _index(who, "seq_off", seq_off, B + 1, q)
-    text, keep2 = _index(who, "text_len", text_len, B, q)
+    seq_off = _index(who, "seq_off", seq_off, B + 1, q)
+    if text_len is not None:
+        text_len = _index(who, "text_len", text_len, B, q)
     o = _out(who, out, q)
     q, k, v = _heads(q), _heads(k), _heads(v)
     (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
-    _call(q, "vle_op_window_attention", dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, o.data_ptr(), off, text, rows, B, H, Hkv,
+    _call(q, "vle_op_window_attention", dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, o.data_ptr(), seq_off.data_ptr(),
+          None if text_len is None else text_len.data_ptr(), rows, B, H, Hkv,
           dh, window, sinks, dh ** -0.5 if scale is None else scale, out is None)
     return o
 
@@ -512,12 +508,14 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     if seq_off is None and rows != B:
         _refuse(who, "without seq_off there is one row per sequence")
     dt = _operands(who, k, v, k_pages, v_pages)
-    at, keep1 = _index(who, "start", start, B, k)
-    off, keep2 = _index(who, "seq_off", seq_off, B + 1, k)
+    start = _index(who, "start", start, B, k)
+    if seq_off is not None:
+        seq_off = _index(who, "seq_off", seq_off, B + 1, k)
     k, v = _heads(k), _heads(v)
     (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
     _call(k, "vle_op_paged_kv_write", dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, k_pages.data_ptr(), v_pages.data_ptr(),
-          None if mass is None else mass.data_ptr(), page_table.data_ptr(), at, off, rows, B, Hkv, dh, n_pages, W, ps)
+          None if mass is None else mass.data_ptr(), page_table.data_ptr(), start.data_ptr(), None if seq_off is None else seq_off.data_ptr(), rows,
+          B, Hkv, dh, n_pages, W, ps)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -544,15 +542,16 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if q.shape != (B, H, dh) or Hkv < 1 or H < 1 or H % Hkv:
         _refuse(who, "q must be (B, H, dh): the table's sequences, the pages' head size, a multiple of their heads")
     dt = _operands(who, q, k_pages, v_pages)
-    n, keep1 = _index(who, "lengths", lengths, B, q)
-    text, keep2 = _index(who, "text_len", text_len, B, q)
+    lengths = _index(who, "lengths", lengths, B, q)
+    if text_len is not None:
+        text_len = _index(who, "text_len", text_len, B, q)
     o = _out(who, out, q)
     q = _heads(q)
     qr, qh, _ = q.stride()
-    room = _paged_decode_workspace(dt, B, H, Hkv, dh, W, ps, window, sinks, text is not None, mass is not None)
+    room = _paged_decode_workspace(dt, B, H, Hkv, dh, W, ps, window, sinks, text_len is not None, mass is not None)
     ws = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None  # per call: two calls, or two graphs, share none
-    _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), n, text,
-          None if mass is None else mass.data_ptr(), ws.data_ptr() if room else None, room, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
+    _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+          lengths.data_ptr(), None if text_len is None else text_len.data_ptr(), None if mass is None else mass.data_ptr(), ws.data_ptr() if room else None, room, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
           dh ** -0.5 if scale is None else scale)
     return o
 
@@ -575,10 +574,11 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     if budget < 1:
         _refuse(who, "budget must be 1 at least")
     dt = _operands(who, k_pages, v_pages)
-    n, keep1 = _index(who, "lengths", lengths, B, k_pages)
-    text, keep2 = _index(who, "text_len", text_len, B, k_pages)
+    lengths = _index(who, "lengths", lengths, B, k_pages)
+    if text_len is not None:
+        text_len = _index(who, "text_len", text_len, B, k_pages)
     kept = page_table.new_empty((B, Hkv, budget))
     left = page_table.new_empty((B,))
-    _call(k_pages, "vle_op_kv_evict", dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), n, text, kept.data_ptr(),
-          left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget, recent, sinks)
+    _call(k_pages, "vle_op_kv_evict", dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+          None if text_len is None else text_len.data_ptr(), kept.data_ptr(), left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget, recent, sinks)
     return kept, left
