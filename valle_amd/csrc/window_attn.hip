@@ -33,7 +33,7 @@ constexpr float WA_DEFER = 8.f;  // exp2-domain growth of a row's maximum below 
 // (late ones, which see most without a window, first), so that neighbours read the same keys; `seq` = -1: no sequence is left for this item and
 // `rest` counts the items past the last one.
 struct Place {
-  int h, seq, off, len, q0, rest;
+  int h, seq, off, len, text, q0, rest;
 };
 template <int QB>
 __device__ inline Place place_of(const WindowAttnArgs& a) {
@@ -47,8 +47,9 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
   int at = item - p.h * per_head;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int off = 0, len = 0;
+    int off = 0, len = 0, text = 0;
     if (b < a.B) {
+      if (a.text_len) text = a.text_len[b];  // (with the offsets, not a round trip to memory later)
       off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
       len = (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
     }
@@ -65,6 +66,7 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
       p.seq = b0 + l;
       p.off = __builtin_amdgcn_readlane(off, l);
       p.len = __builtin_amdgcn_readlane(len, l);
+      p.text = min(max(__builtin_amdgcn_readlane(text, l), 0), p.len);
       p.q0 = (__builtin_amdgcn_readlane(inc, l) - 1 - at) * QB;
       p.rest = 0;
       return p;
@@ -72,7 +74,7 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
     at -= __builtin_amdgcn_readlane(inc, 63);
   }
   p.seq = -1;
-  p.off = p.len = p.q0 = 0;
+  p.off = p.len = p.text = p.q0 = 0;
   p.rest = at;
   return p;
 }
@@ -108,55 +110,60 @@ __device__ inline Sight sight_of(int i, int text, int window, int sinks) {
   return s;
 }
 
-__device__ inline float wa_elem(const void* p, int64_t i, bool bf) { return bf ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i]; }
-
-// One row over its visible keys alone, by one wave: 64 keys at a time, a lane the score of one, then two elements of the output.
+// One row over its visible keys alone, by one wave: 64 keys at a time, a lane the score of one, then two elements of the output as the average so far.
 template <typename T>
 __device__ inline void exact_row(const WindowAttnArgs& a, int h, int off, int i, int text, int len) {
 #pragma clang fp contract(off)  // score - m must be the difference of two rounded scores: 0 for the largest, whatever its size
-  constexpr bool BF = sizeof(T) == 2;
+  constexpr int VE = Elem<T>::VEC;
   const int lane = threadIdx.x & 63, hk = h / (a.H / a.Hkv);
   const Sight see = sight_of(i, text, a.window, a.sinks);
-  const int64_t qo = (int64_t)(off + i) * a.q_row + (int64_t)h * a.q_head;
-  auto score = [&](int j) -> float {
-    const int64_t ko = (int64_t)(off + j) * a.k_row + (int64_t)hk * a.k_head;
-    float s = 0.f;
-    for (int e = 0; e < a.dh; ++e) s = fmaf(wa_elem(a.q, qo + e, BF), wa_elem(a.k, ko + e, BF), s);
-    return s * a.sl2;
-  };
+  const T* q = (const T*)a.q + (int64_t)(off + i) * a.q_row + (int64_t)h * a.q_head;
+  const T* k = (const T*)a.k + (int64_t)off * a.k_row + (int64_t)hk * a.k_head;
+  const T* v = (const T*)a.v + (int64_t)off * a.v_row + (int64_t)hk * a.v_head;
+  const bool in0 = lane < a.dh, in1 = lane + 64 < a.dh;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  bool bad = false;  // a score that is not a number, or none above -inf
   const int end = min(len, max(see.hd, i + 1));
-  float m = -INFINITY;
-  bool nan = false;
-  for (int j = lane; j < end; j += 64)
-    if (see.sees(j)) {
-      const float s = score(j);
-      nan |= s != s;
-      m = fmaxf(m, s);
-    }
-  m = wave_max(m);
-  if (__any(nan)) m = __builtin_nanf("");
-  float l = 0.f;
-  for (int j = lane; j < end; j += 64)
-    if (see.sees(j)) l += __builtin_amdgcn_exp2f(score(j) - m);
-  l = wave_sum(l);
-  float o0 = 0.f, o1 = 0.f;
-  for (int j0 = 0; j0 < end; j0 += 64) {
+  for (int j0 = 0; j0 < end && !bad; j0 += 64) {
     const int j = j0 + lane;
-    const bool vis = j < end && see.sees(j);
-    const float p = vis ? __builtin_amdgcn_exp2f(score(j) - m) / l : 0.f;
+    const bool vis = (j < end) & see.sees(j);
+    if (!__any(vis)) continue;
+    float s = -INFINITY;
+    if (vis) {
+      float sum = 0.f;
+      for (int e = 0; e < a.dh; e += VE) {
+        float x[VE], y[VE];
+        load_vec16(q + e, x);
+        load_vec16(k + (int64_t)j * a.k_row + e, y);
+#pragma unroll
+        for (int u = 0; u < VE; ++u) sum = fmaf(x[u], y[u], sum);
+      }
+      s = sum * a.sl2;
+    }
+    bad = __any(s != s);
+    const float mn = fmaxf(m, wave_max(s));
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float p = __builtin_amdgcn_exp2f(s - ref);
+    const float was = l * __builtin_amdgcn_exp2f(m - ref), now = was + wave_sum(p);
+    m = mn;
+    l = now;
+    if (now == 0.f) continue;  // nothing but -inf so far
+    o0 *= was / now;
+    o1 *= was / now;
     unsigned long long todo = __ballot(vis);
     while (todo) {
       const int t = __builtin_ctzll(todo);
       todo &= todo - 1;
-      const float w = readlane_f32(p, t);
-      const int64_t vo = (int64_t)(off + j0 + t) * a.v_row + (int64_t)hk * a.v_head;
-      if (lane < a.dh) o0 = fmaf(w, wa_elem(a.v, vo + lane, BF), o0);
-      if (lane + 64 < a.dh) o1 = fmaf(w, wa_elem(a.v, vo + lane + 64, BF), o1);
+      const float w = readlane_f32(p, t) / now;
+      const T* row = v + (int64_t)(j0 + t) * a.v_row;
+      if (in0) o0 = fmaf(w, Elem<T>::to_f32(row[lane]), o0);
+      if (in1) o1 = fmaf(w, Elem<T>::to_f32(row[lane + 64]), o1);
     }
   }
+  if (bad | (l == 0.f)) o0 = o1 = __builtin_nanf("");
   T* op = (T*)a.out + ((int64_t)(off + i) * a.H + h) * a.dh;
-  if (lane < a.dh) store_elem<T>(op + lane, o0);
-  if (lane + 64 < a.dh) store_elem<T>(op + lane + 64, o1);
+  if (in0) store_elem<T>(op + lane, o0);
+  if (in1) store_elem<T>(op + lane + 64, o1);
 }
 
 // Rows that no sequence holds, `rest`-th run of them.
@@ -223,7 +230,7 @@ struct Stager {
 
 // ---- bf16 --------------------------------------------------------------------------------------------------------------------------
 // 4 waves, QW query fragments of 16 rows each; 64-key tiles of K and V go global -> LDS by DMA into one of two buffers while the other is
-// multiplied; V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the matrix pipe (an all-ones
+// multiplied (a third buffer changed nothing); V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the matrix pipe (an all-ones
 // row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16 (8 bits: 2^-9 of each weight, which
 // averages out over the keys and stays below the output's own rounding).
 template <int DHT, int QW>
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
   const int wu = __builtin_amdgcn_readfirstlane(w);
   const int len = pl.len, q0 = pl.q0, dh = a.dh, hk = pl.h / (a.H / a.Hkv);
-  const int text = a.text_len ? min(max(a.text_len[pl.seq], 0), len) : 0;
+  const int text = pl.text;
   const Tiles ti = tiles_of<TK>(q0, min(q0 + QB, len) - 1, text, a.window, a.sinks);
   const bf16_t* kb = (const bf16_t*)a.k + (int64_t)pl.off * a.k_row + (int64_t)hk * a.k_head;
   const bf16_t* vb = (const bf16_t*)a.v + (int64_t)pl.off * a.v_row + (int64_t)hk * a.v_head;
@@ -258,7 +265,6 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
       wa_u32x4 x = {0u, 0u, 0u, 0u};
       if (ks * 32 + g * 8 < dh) x = *reinterpret_cast<const wa_u32x4*>(qp + ks * 32 + g * 8);
       qf[f][ks] = __builtin_bit_cast(wa_bf16x8, x);
-      asm volatile("" : "+v"(qf[f][ks]));  // waited for here, once: a wait at the first use would stand inside the loop and take the tiles in flight with it
     }
   }
 
@@ -278,6 +284,11 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
   const Stager<bf16_t, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
   stage_k(key0(0), dh, smem);
   stage_v(key0(0), dh, smem + HALF);
+  // the queries are waited for here, once: a wait at their first use would stand inside the loop and take the tiles in flight with it
+#pragma unroll
+  for (int f = 0; f < QW; ++f)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[f][ks]));
   for (int t = 0; t < ti.tt; ++t) {
     const int kt0 = key0(t);
     const unsigned char* Ks = smem + (t & 1) * BUF;
@@ -460,7 +471,7 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
   const int wu = __builtin_amdgcn_readfirstlane(w);
   const int len = pl.len, q0 = pl.q0, dh = a.dh, hk = pl.h / (a.H / a.Hkv);
-  const int text = a.text_len ? min(max(a.text_len[pl.seq], 0), len) : 0;
+  const int text = pl.text;
   const Tiles ti = tiles_of<TK>(q0, min(q0 + QB, len) - 1, text, a.window, a.sinks);
   const float* kb = (const float*)a.k + (int64_t)pl.off * a.k_row + (int64_t)hk * a.k_head;
   const float* vb = (const float*)a.v + (int64_t)pl.off * a.v_row + (int64_t)hk * a.v_head;
@@ -473,7 +484,6 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   for (int t = 0; t < KT; ++t) {
     qf[t] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
     if (t * 16 + g * 4 < dh) qf[t] = *reinterpret_cast<const wa_f32x4*>(qp + t * 16 + g * 4);
-    asm volatile("" : "+v"(qf[t]));  // as in the bf16 kernel
   }
   const float sl2 = a.sl2;
   float m = -INFINITY, l = 0.f;
@@ -485,6 +495,8 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   const Stager<float, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
   stage_k(key0(0), dh, smem);
   stage_v(key0(0), dh, smem + HALF);
+#pragma unroll
+  for (int t = 0; t < KT; ++t) asm volatile("" : "+v"(qf[t]));  // as in the bf16 kernel
   for (int t = 0; t < ti.tt; ++t) {
     const int kt0 = key0(t);
     const unsigned char* Ks = smem + (t & 1) * BUF;
@@ -497,16 +509,22 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
       stage_v(key0(t + 1), dh, nb + HALF);
     }
     if (!__any(see.any(kt0, TK))) continue;
-    wa_f32x4 s[2];
+    wa_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    wa_f32x4 ka[2][2];  // [buffer][16-key tile]: the next 16 dims' fragments are read while these are multiplied
+    auto read_k = [&](wa_f32x4 (&d)[2], int t4) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      s[kt] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < 2; ++kt) d[kt] = *reinterpret_cast<const wa_f32x4*>(Ks + (kt * 16 + c) * ROW + (((t4 * 4 + g) ^ wa_key<NV>(c)) << 4));
+    };
+    read_k(ka[0], 0);
 #pragma unroll
-      for (int t4 = 0; t4 < KT; ++t4) {
-        const wa_f32x4 ka = *reinterpret_cast<const wa_f32x4*>(Ks + (kt * 16 + c) * ROW + (((t4 * 4 + g) ^ wa_key<NV>(c)) << 4));
+    for (int t4 = 0; t4 < KT; ++t4) {
+      if (t4 + 1 < KT) read_k(ka[(t4 + 1) & 1], t4 + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[u], qf[t4][u], s[kt], 0, 0, 0);
-      }
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[t4 & 1][kt][u], qf[t4][u], s[kt], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
     const bool unmasked = __all(see.all(kt0, TK));
     float mt = -INFINITY;
@@ -535,34 +553,38 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
 #pragma unroll
       for (int j = 0; j < DPL; ++j) o[j] *= alpha;
     }
+    auto read_v = [&](float (&vv)[DPL], int n) {  // this lane's dims of key 4 g + n % 4 of score tile n / 4
+      const int key = (n >> 2) * 16 + g * 4 + (n & 3);
+      const unsigned char* row = Vs + key * ROW;
+      if constexpr (A4 == 4) {
+        const wa_f32x4 x = *reinterpret_cast<const wa_f32x4*>(row + ((c ^ wa_key<NV>(key)) << 4));
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+        for (int j = 0; j < 4; ++j) vv[j] = x[j];
+        if constexpr (B4 == 4) {
+          const wa_f32x4 y = *reinterpret_cast<const wa_f32x4*>(row + (((16 + c) ^ wa_key<NV>(key)) << 4));
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = kt * 16 + g * 4 + r;
-        const unsigned char* row = Vs + key * ROW;
-        float vv[DPL];
-        if constexpr (A4 == 4) {
-          const wa_f32x4 x = *reinterpret_cast<const wa_f32x4*>(row + ((c ^ wa_key<NV>(key)) << 4));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vv[j] = x[j];
-          if constexpr (B4 == 4) {
-            const wa_f32x4 y = *reinterpret_cast<const wa_f32x4*>(row + (((16 + c) ^ wa_key<NV>(key)) << 4));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) vv[4 + j] = y[j];
-          } else if constexpr (B4 == 2) {
-            const wa_f32x2 y = *reinterpret_cast<const wa_f32x2*>(row + (((16 + (c >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
-            vv[4] = y[0];
-            vv[5] = y[1];
-          }
-        } else {
-          const wa_f32x2 x = *reinterpret_cast<const wa_f32x2*>(row + (((c >> 1) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
-          vv[0] = x[0];
-          vv[1] = x[1];
+          for (int j = 0; j < 4; ++j) vv[4 + j] = y[j];
+        } else if constexpr (B4 == 2) {
+          const wa_f32x2 y = *reinterpret_cast<const wa_f32x2*>(row + (((16 + (c >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
+          vv[4] = y[0];
+          vv[5] = y[1];
         }
-#pragma unroll
-        for (int j = 0; j < DPL; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[j], s[kt][r], o[j], 0, 0, 0);
+      } else {
+        const wa_f32x2 x = *reinterpret_cast<const wa_f32x2*>(row + (((c >> 1) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3));
+        vv[0] = x[0];
+        vv[1] = x[1];
       }
+    };
+    float vv[2][DPL];  // the next key's elements are read while these are multiplied
+    read_v(vv[0], 0);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (n < 7) read_v(vv[(n + 1) & 1], n + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[n & 1][j], s[n >> 2][n & 3], o[j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   l = rows4_sum(l);
   bool odd = false;
