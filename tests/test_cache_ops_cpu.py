@@ -35,6 +35,9 @@ I32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     (dict(out=torch.zeros(6, 4, 8)), ValueError),
     (dict(out=torch.zeros(4, 6, 16).transpose(0, 1)), ValueError),
     (dict(q=torch.zeros(6, 4, 16, requires_grad=True)), RuntimeError),
+    (dict(window=-1), ValueError),
+    (dict(window=2 ** 32 + 5), ValueError),  # would arrive as 5 in 32 bits
+    (dict(sinks=2 ** 31), ValueError),
     (dict(), AssertionError),  # no CPU path
 ])
 def test_window_attention_refuses(kw, err):
@@ -87,8 +90,11 @@ def test_cache_operators_refuse_bad_rows():
     mass = torch.zeros(3, 2, 8)
     with pytest.raises(ValueError):
         ops.kv_evict(mass=None, lengths=I32(1, 1), budget=4, **c)
+    for kw in (dict(budget=0), dict(budget=-3), dict(budget=2 ** 32 + 4), dict(budget=4, recent=-1), dict(budget=4, sinks=2 ** 32)):
+        with pytest.raises(ValueError):
+            ops.kv_evict(mass=mass, lengths=I32(1, 1), **kw, **c)
     with pytest.raises(ValueError):
-        ops.kv_evict(mass=mass, lengths=I32(1, 1), budget=0, **c)
+        ops.paged_decode_attention(torch.zeros(2, 4, 16), lengths=I32(1, 1), window=2 ** 33, **c)
     with pytest.raises(ValueError):
         ops.kv_evict(mass=mass, lengths=I32(1, 1), budget=4, **dict(c, v_pages=c["k_pages"]))
 
@@ -132,6 +138,7 @@ def test_c_workspace_query():
     wide, bounded = (lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8192, 16, w, 4, 0, 1) for w in (0, 500))
     assert bounded < wide // 50 and lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 64, 8192, 16, 500, 4, 1, 1) > wide // 2
     assert lib.vle_op_paged_decode_workspace_bytes(1, 1, 16, 16, 60, 8, 16, 0, 0, 0, 0) == _lib.VLE_EINVAL
+    assert lib.vle_op_paged_decode_workspace_bytes(1, 0, 16, 16, 64, 8192, 16, 0, 0, 0, 1) == 0  # no sequence at all
 
 
 def _c_write(dtype=0, rows=2, B=2, Hkv=2, dh=16, n_pages=3, W=2, ps=8, off=None, k=P, row=32):

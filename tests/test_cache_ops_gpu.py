@@ -104,6 +104,30 @@ def test_window_attention(dtype, lens, text, H, Hkv, dh, window, sinks):
     near(got, *window_ref(q, k, v, off, text, window, sinks), "window")
 
 
+@pytest.mark.parametrize("B", [65, 300])
+def test_window_attention_and_write_of_many_short_sequences(B):
+    """More sequences than a wave has lanes, empty ones among them: attention of their prompts, the write of their keys, a step over the cache."""
+    g, H, dh, ps = gen(B), 2, 32, 8
+    lens = torch.randint(0, 9, (B,), generator=g).tolist()
+    off, text = offsets(lens), [min(2, n) for n in lens]
+    q, k, v = (rnd(g, off[-1], H, dh, dtype=torch.bfloat16) for _ in range(3))
+    got = ops.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(off), window=3, sinks=1, text_len=i32(text))
+    near(got, *window_ref(q, k, v, off, text, 3, 1), "window")
+    pool = Pool(g, lens, H, dh, ps, torch.bfloat16)
+    kp, vp, table, mass = pool.device()
+    kp.fill_(float("nan")), vp.fill_(float("nan"))
+    ops.paged_kv_write(k.to(DEV), v.to(DEV), kp, vp, table, i32([0] * B), seq_off=i32(off), mass=mass)
+    for b in range(B):
+        page, slot = pool.at(b)
+        pool.k[page, :, slot], pool.v[page, :, slot], pool.mass[page, :, slot] = k[off[b]:off[b + 1]], v[off[b]:off[b + 1]], 0.0
+    same = lambda a, w: bool(((a.cpu() == w) | (a.cpu().isnan() & w.isnan())).all())  # noqa: E731
+    assert same(kp, pool.k) and same(vp, pool.v) and same(mass, pool.mass)
+    one = rnd(g, B, H, dh, dtype=torch.bfloat16)
+    out, tol, add, add_tol = decode_ref(pool, one, text, 3, 1)
+    near(ops.paged_decode_attention(one.to(DEV), kp, vp, table, i32(lens), window=3, sinks=1, text_len=i32(text), mass=mass), out, tol, "step")
+    near(mass, pool.mass.to(F64) + add, add_tol + 2.0 ** -22, "mass")
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_window_attention_views_and_rows_of_no_sequence(dtype):
     """q / k / v as slices of one packed qkv, keys and values of one head broadcast over all, operands off the 16-byte grid; sequences that start behind row 0 and end

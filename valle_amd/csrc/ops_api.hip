@@ -292,6 +292,7 @@ static const char* heads_fault(int dtype, int32_t nhead, int32_t nhead_kv, int32
   if (dtype != DT_F32 && dtype != DT_BF16) return "dtype must be f32 or bf16";
   if (nhead < 1 || nhead_kv < 1 || nhead % nhead_kv) return "nhead must be a multiple of nhead_kv";
   if (nhead / nhead_kv > 256) return "at most 256 query heads share a key-value head";
+  if (nhead > 65535) return "at most 65535 heads";
   if (dh < 8 || dh > 128 || dh % 8) return "head size must be a multiple of 8 up to 128";
   return nullptr;
 }
@@ -343,7 +344,8 @@ extern "C" int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int
   const char* op = "vle_op_paged_kv_write";
   if (const char* e = heads_fault(dtype, nhead_kv, nhead_kv, dh)) return op_refuse(op, e);
   if (const char* e = cache_fault(B, nhead_kv, dh, n_pages, table_width, page_size)) return op_refuse(op, e);
-  if (rows < 0 || rows > 0x7fff0000 || (!seq_off_dev && rows != B)) return op_refuse(op, "without seq_off there is one row per sequence");
+  if (rows < 0 || rows > (1 << 25)) return op_refuse(op, "0 to 2^25 rows");
+  if (!seq_off_dev && rows != B) return op_refuse(op, "without seq_off there is one row per sequence");
   if (rows == 0 || B == 0) return VLE_OK;
   if (!k || !v || !k_pages || !v_pages || !page_table_dev || !start_dev) return op_refuse(op, "null operand");
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || !vec_strides(dtype, k_row, k_head) ||
@@ -363,6 +365,7 @@ extern "C" int64_t vle_op_paged_decode_workspace_bytes(int dtype, int32_t B, int
   if (!e) e = cache_fault(B, nhead_kv, dh, 1, table_width, page_size);
   if (!e && (window < 0 || sinks < 0)) e = "window and sinks must not be negative";
   if (e) return op_refuse(op, e);
+  if (B == 0) return 0;
   const PagedDecodePlan p = paged_decode_plan(dtype, B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, has_text != 0, has_mass != 0);
   return (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
 }

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs a) {
     int ended = 0;
     for (int i = lane; i < a.B; i += 64) ended += a.seq_off[i + 1] <= row;
     b = wave_sum_i(ended);
-    if (b >= a.B || row < a.seq_off[b]) return;  // behind the last sequence or ahead of the first
+    if (b >= a.B || row < a.seq_off[b] || row >= a.seq_off[b + 1]) return;  // behind the last sequence or ahead of the first
     at = (int)row - a.seq_off[b];
   }
   const int64_t pos = (int64_t)a.start[b] + at;

@@ -45,21 +45,43 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
   Place p;
   p.h = item / per_head;
   int at = item - p.h * per_head;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    int off = 0, len = 0, text = 0;
-    if (b < a.B) {
-      if (a.text_len) text = a.text_len[b];  // (with the offsets, not a round trip to memory later)
-      off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
-      len = (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
-    }
-    const int runs = (len + QB - 1) / QB;
-    int inc = runs;
+  auto rows_of = [&](int b, int& off) {  // clamped to the rows there are, whatever the offsets say
+    off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
+    return (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
+  };
+  auto scan = [&](int x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += t;
+      const int t = __shfl_up(x, o, 64);
+      if (lane >= o) x += t;
     }
+    return x;
+  };
+  int lo = 0, hi = a.B;
+  const int per = (a.B + 63) >> 6;
+  if (per > 1) {  // many sequences: which lane's share of them holds the item
+    int sum = 0, off;
+    for (int b = lane * per; b < min((lane + 1) * per, a.B); ++b) sum += (rows_of(b, off) + QB - 1) / QB;
+    const int inc = scan(sum);
+    const unsigned long long past = __ballot(at < inc);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      at -= __builtin_amdgcn_readlane(inc - sum, l);
+      lo = l * per;
+      hi = min(lo + per, a.B);
+    } else {
+      at -= __builtin_amdgcn_readlane(inc, 63);
+      hi = 0;
+    }
+  }
+  for (int b0 = lo; b0 < hi; b0 += 64) {
+    const int b = b0 + lane;
+    int off = 0, len = 0, text = 0;
+    if (b < hi) {
+      if (a.text_len) text = a.text_len[b];  // (with the offsets, not a round trip to memory later)
+      len = rows_of(b, off);
+    }
+    const int inc = scan((len + QB - 1) / QB);
     const unsigned long long past = __ballot(at < inc);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -619,7 +641,7 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
   const bool wide = !f32 && items(128) * a.H >= 1024;
   const int64_t n = items(wide ? 128 : 64) * a.H;
-  if (n > 0x7fffffff) return -1;
+  if (n > 0xffffff) return -1;  // 2^32 work items
   const dim3 grid((unsigned)n), block(256);
 #define VLE_WA(DHT)                                                                             \
   do {                                                                                          \

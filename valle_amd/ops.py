@@ -383,6 +383,13 @@ def _refuse(who: str, what: str):
     raise ValueError(f"{who}: {what}")
 
 
+def _count(who: str, name: str, v: int) -> int:
+    """v, which a C entry takes in 32 bits."""
+    if not 0 <= v < 1 << 31:
+        _refuse(who, f"{name} must be 0 to 2^31 - 1, got {v}")
+    return v
+
+
 def _operands(who: str, first: torch.Tensor, *others: torch.Tensor) -> int:
     """One device, one type, no gradient asked for; -> the type's code."""
     what, where, grad = first.dtype, first.get_device(), first.requires_grad
@@ -419,9 +426,9 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 
 def _out(who: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return like.new_empty(like.shape)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() or out.data_ptr() % 16:
-        _refuse(who, "out must be a contiguous tensor like q, on 16 bytes")
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if (out.data_ptr() == like.data_ptr() and like.numel()) or out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() or out.data_ptr() % 16:
+        _refuse(who, "out must be a contiguous tensor like q, on 16 bytes, and not q itself")
     return out
 
 
@@ -441,6 +448,8 @@ def _pages(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: t
             raise TypeError(f"{who}: mass must be float32, got {mass.dtype}")
         if mass.shape != shape[:3] or not mass.is_contiguous() or mass.get_device() != where:
             _refuse(who, "mass must be a contiguous (n_pages, heads, page_size) tensor on the pages' device")
+    if shape[0] >> 31 or page_table.numel() >> 31:
+        _refuse(who, "pools and tables have fewer than 2^31 pages")
     return (*shape, *page_table.shape)
 
 
@@ -486,7 +495,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
     _call(q, "vle_op_window_attention", dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, o.data_ptr(), seq_off.data_ptr(),
           None if text_len is None else text_len.data_ptr(), rows, B, H, Hkv,
-          dh, window, sinks, dh ** -0.5 if scale is None else scale, out is None)
+          dh, _count(who, "window", window), _count(who, "sinks", sinks), dh ** -0.5 if scale is None else scale, out is None)
     return o
 
 
@@ -548,6 +557,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     o = _out(who, out, q)
     q = _heads(q)
     qr, qh, _ = q.stride()
+    _count(who, "window", window)
+    _count(who, "sinks", sinks)
     room = _paged_decode_workspace(dt, B, H, Hkv, dh, W, ps, window, sinks, text_len is not None, mass is not None)
     ws = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None  # per call: two calls, or two graphs, share none
     _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
@@ -571,14 +582,15 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
     if k_pages.data_ptr() == v_pages.data_ptr() and k_pages.numel():
         _refuse(who, "keys and values need pages of their own")
-    if budget < 1:
+    if _count(who, "budget", budget) < 1:
         _refuse(who, "budget must be 1 at least")
     dt = _operands(who, k_pages, v_pages)
     lengths = _index(who, "lengths", lengths, B, k_pages)
     if text_len is not None:
         text_len = _index(who, "text_len", text_len, B, k_pages)
     kept = page_table.new_empty((B, Hkv, budget))
-    left = page_table.new_empty((B,))
+    left = torch.empty_like(lengths)
     _call(k_pages, "vle_op_kv_evict", dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-          None if text_len is None else text_len.data_ptr(), kept.data_ptr(), left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget, recent, sinks)
+          None if text_len is None else text_len.data_ptr(), kept.data_ptr(), left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget,
+          _count(who, "recent", recent), _count(who, "sinks", sinks))
     return kept, left
