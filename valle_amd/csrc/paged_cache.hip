@@ -453,7 +453,10 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
   const int64_t slots = 256 * (dh <= 64 ? 5 : 3);
   p.nsplit = 1;
   p.nw = groups < 512 && ng <= 8 ? 8 : 4;  // 8 waves: their outputs fit 32 KB of LDS for up to 8 heads
-  if (groups < 512 && p.tiles > 8 * p.nw) {
+  // One workgroup a head takes 7 us per 1000 keys of 64 (a CU alone pulls about 40 GB/s), the join costs 3 us and a launch on the host: one sequence of
+  // 16 heads of 64 is faster unsplit up to 1040 keys (10.7 / 14.0 us a call), split from 1500 on (13.6 / 13.8; 13.8 / 10.0 in a graph).  A group for
+  // every CU needs no split yet at 2000 keys (16 sequences, 16 heads: 27 / 31 us).
+  if (groups < 512 && p.tiles > (groups < 256 ? 5 : 16) * p.nw) {
     p.nw = 4;
     p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), std::max((int64_t)1, slots / groups));
   }

@@ -478,20 +478,22 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 // The same walk on v_mfma_f32_16x16x4_f32 (exact fp32 products, 1/16 of the bf16 rate): 64 query rows, 32-key tiles.  A 16-byte fragment of
 // K feeds four products (contraction slot g of product u is dim 16 t + 4 g + u); V^T needs no transpose: product j of key r takes V[4 g + r][dim(c, j)],
 // with dim(c, j) the j-th of the up to 8 elements that lane c reads of a row.
-template <int DHT>
-__global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) {
+// NG = 2: two groups of 4 waves share the rows and take every other tile each; their halves are joined at the end.
+template <int DHT, int NG>
+__global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArgs a) {
   constexpr int QB = 64, TK = 32, NV = DHT / 4, ROW = DHT * 4, KT = DHT / 16, DPL = DHT / 16;
   constexpr int HALF = TK * ROW, BUF = 2 * HALF;
   constexpr int A4 = DPL >= 4 ? 4 : 2;           // elements of a lane's first chunk of a V row, and of its second
   constexpr int B4 = DPL - A4;                   // (DHT 32: 2, 64: 4, 96: 4 + 2, 128: 4 + 4)
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BUF];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * NG * BUF];
   const Place pl = place_of<QB>(a);
   if (pl.seq < 0) {
     if (a.zero_rest) zero_rows<float, QB>(a, pl.h, pl.rest);
     return;
   }
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int wu = __builtin_amdgcn_readfirstlane(w);
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = w8 & 3, group = NG == 2 ? w8 >> 2 : 0;
+  unsigned char* const mine = smem + group * 2 * BUF;
   const int len = pl.len, q0 = pl.q0, dh = a.dh, hk = pl.h / (a.H / a.Hkv);
   const int text = pl.text;
   const Tiles ti = tiles_of<TK>(q0, min(q0 + QB, len) - 1, text, a.window, a.sinks);
@@ -514,22 +516,26 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
   for (int j = 0; j < DPL; ++j) o[j] = wa_f32x4{0.f, 0.f, 0.f, 0.f};
   auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
 
-  const Stager<float, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
-  stage_k(key0(0), dh, smem);
-  stage_v(key0(0), dh, smem + HALF);
+  const Stager<float, TK, NV> stage_k(kb, a.k_row, len, dh, w), stage_v(vb, a.v_row, len, dh, w);
+  if (group < ti.tt) {
+    stage_k(key0(group), dh, mine);
+    stage_v(key0(group), dh, mine + HALF);
+  }
 #pragma unroll
   for (int t = 0; t < KT; ++t) asm volatile("" : "+v"(qf[t]));  // as in the bf16 kernel
-  for (int t = 0; t < ti.tt; ++t) {
-    const int kt0 = key0(t);
-    const unsigned char* Ks = smem + (t & 1) * BUF;
+  for (int t0 = 0; t0 < ti.tt; t0 += NG) {
+    const int t = t0 + group;
+    const unsigned char* Ks = mine + (t0 / NG & 1) * BUF;
     const unsigned char* Vs = Ks + HALF;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (t + 1 < ti.tt) {
-      unsigned char* nb = smem + ((t + 1) & 1) * BUF;
-      stage_k(key0(t + 1), dh, nb);
-      stage_v(key0(t + 1), dh, nb + HALF);
+    if (t + NG < ti.tt) {
+      unsigned char* nb = mine + (t0 / NG + 1 & 1) * BUF;
+      stage_k(key0(t + NG), dh, nb);
+      stage_v(key0(t + NG), dh, nb + HALF);
     }
+    if (t >= ti.tt) continue;
+    const int kt0 = key0(t);
     if (!__any(see.any(kt0, TK))) continue;
     wa_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     wa_f32x4 ka[2][2];  // [buffer][16-key tile]: the next 16 dims' fragments are read while these are multiplied
@@ -609,6 +615,28 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
     }
   }
   l = rows4_sum(l);
+  if constexpr (NG == 2) {  // lane by lane: both groups hold the same rows and elements in the same places
+    __syncthreads();        // the tiles are done with
+    float* part = reinterpret_cast<float*>(smem) + w * 64 + lane;
+    constexpr int N = 4 * 64;
+    if (group == 1) {
+      part[0] = m;
+      part[N] = l;
+#pragma unroll
+      for (int j = 0; j < DPL; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) part[(2 + 4 * j + r) * N] = o[j][r];
+    }
+    __syncthreads();
+    if (group == 1) return;
+    const float m1 = part[0], mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f((m - ref) * sl2), f1 = __builtin_amdgcn_exp2f((m1 - ref) * sl2);
+    l = l * f0 + part[N] * f1;
+#pragma unroll
+    for (int j = 0; j < DPL; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[j][r] = o[j][r] * f0 + part[(2 + 4 * j + r) * N] * f1;
+  }
   bool odd = false;
   float* op = (float*)a.out + ((int64_t)(pl.off + i) * a.H + pl.h) * dh;
 #pragma unroll
@@ -629,7 +657,7 @@ __global__ __launch_bounds__(256) void window_attn_f32_kernel(WindowAttnArgs a) 
     while (again) {
       const int t = __builtin_ctzll(again);
       again &= again - 1;
-      exact_row<float>(a, pl.h, pl.off, q0 + wu * 16 + t, text, len);
+      exact_row<float>(a, pl.h, pl.off, q0 + w * 16 + t, text, len);
     }
   }
 }
@@ -641,11 +669,15 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
   const bool wide = !f32 && items(128) * a.H >= 1024;
   const int64_t n = items(wide ? 128 : 64) * a.H;
+  // fp32, at most about one workgroup a CU: a second group of waves halves each one's walk (one sequence of 1025 rows, 16 heads of 64: 66 -> 58 us;
+  // 4 key-value heads of 128, window 300: 51 -> 40).  With more, the tiles of both groups keep a second workgroup off the CU (window_fp32 57 -> 65 us).
+  const bool pair = f32 && n <= 384;
   if (n > 0xffffff) return -1;  // 2^32 work items
   const dim3 grid((unsigned)n), block(256);
 #define VLE_WA(DHT)                                                                             \
   do {                                                                                          \
-    if (f32) hipLaunchKernelGGL((window_attn_f32_kernel<DHT>), grid, block, 0, st, a);          \
+    if (pair) hipLaunchKernelGGL((window_attn_f32_kernel<DHT, 2>), grid, dim3(512), 0, st, a);   \
+    else if (f32) hipLaunchKernelGGL((window_attn_f32_kernel<DHT, 1>), grid, block, 0, st, a);   \
     else if (wide) hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 2>), grid, block, 0, st, a); \
     else hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 1>), grid, block, 0, st, a);          \
   } while (0)
