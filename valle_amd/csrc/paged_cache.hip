@@ -676,33 +676,30 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
 // many bytes but whose lanes walk it alone: 302.
 constexpr int MV_T = 1024, MV_U = 2, MV_TAB = 4096;
 
-template <typename V>
-__device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* kept, const int32_t* tab, const int32_t* sh_tab, int h, int vpr, int e0,
-                                  int width, int len) {
+template <bool CACHED, typename V>  // CACHED: the sequence's pages are in LDS
+__device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* kept, const int32_t* tab, const int32_t (&sh_tab)[MV_TAB], int h, int vpr,
+                                  int e0, int width, int len) {
   const int tid = threadIdx.x, ps = 1 << a.psl, n = a.budget;
   const int64_t page_vecs = (int64_t)a.Hkv * ps * vpr;
   const int rows = MV_T / width, row0 = tid / width, e = e0 + tid % width;  // rows a pass, this thread's and its column
   const bool mine = row0 < rows;
-  auto page_of = [&](int j) { return sh_tab != nullptr ? sh_tab[j >> a.psl] : tab[j >> a.psl]; };
+  auto page_of = [&](int j) { return CACHED ? sh_tab[j >> a.psl] : tab[j >> a.psl]; };
+  auto place = [&](int page, int j) { return pool + (int64_t)page * page_vecs + (int64_t)(h * ps + (j & (ps - 1))) * vpr + e; };
+  // No branch around a load (rows past the end read the last one's, vectors that do not move the pool's first), so that the waits for a chunk can
+  // leave the next one's loads in flight.
   int from[MV_U];
   auto load_kept = [&](int base) {
 #pragma unroll
-    for (int u = 0; u < MV_U; ++u) {
-      const int row = base + u * rows + row0;
-      from[u] = mine && row < n ? kept[row] : -1;
-    }
+    for (int u = 0; u < MV_U; ++u) from[u] = kept[min(base + u * rows + row0, n - 1)];
   };
-  auto place = [&](int page, int j) { return pool + (int64_t)page * page_vecs + (int64_t)(h * ps + (j & (ps - 1))) * vpr + e; };
-  // loads are unconditional (from the pool's first vector where there is nothing to move), so that the waits for them can be counted;
-  // bit u of the result: vector u is to be stored
-  auto load_rows = [&](int base, V (&x)[MV_U]) -> unsigned {
+  auto load_rows = [&](int base, V (&x)[MV_U]) -> unsigned {  // bit u: vector u is to be stored
     unsigned moves = 0;
 #pragma unroll
     for (int u = 0; u < MV_U; ++u) {
       const int row = base + u * rows + row0;
-      const bool go = (from[u] > row) & (from[u] < len);
-      const int sp = go ? page_of(from[u]) : -1, dp = go ? page_of(row) : -1;
-      const bool there = ((unsigned)sp < (unsigned)a.n_pages) & ((unsigned)dp < (unsigned)a.n_pages);
+      const bool go = mine & (row < n) & (from[u] > row) & (from[u] < len);
+      const int sp = page_of(go ? from[u] : 0), dp = page_of(go ? row : 0);
+      const bool there = go & ((unsigned)sp < (unsigned)a.n_pages) & ((unsigned)dp < (unsigned)a.n_pages);
       x[u] = *(there ? place(sp, from[u]) : pool);
       moves |= there ? 1u << u : 0u;
     }
@@ -710,11 +707,8 @@ __device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* ke
   };
   const int step = MV_U * rows;
   auto turn = [&](int base, V (&x)[MV_U], unsigned moves, V (&next)[MV_U]) -> unsigned {
-    unsigned m2 = 0;
-    if (base + step < n) {
-      m2 = load_rows(base + step, next);
-      load_kept(base + 2 * step);
-    }
+    const unsigned m2 = load_rows(base + step, next);
+    load_kept(base + 2 * step);
 #pragma unroll
     for (int u = 0; u < MV_U; ++u) asm volatile("" : "+v"(x[u])::"memory");  // the chunk's loads have returned to this wave
     __syncthreads();
@@ -732,7 +726,7 @@ __device__ inline void evict_move(V* pool, const EvictArgs& a, const int32_t* ke
   load_kept(step);
   for (int base = 0; base < n; base += 2 * step) {
     my = turn(base, x, mx, y);
-    if (base + step < n) mx = turn(base + step, y, my, x);
+    mx = turn(base + step, y, my, x);  // past the end: nothing moves
   }
 }
 
@@ -745,15 +739,16 @@ __global__ __launch_bounds__(MV_T) void kv_evict_move_kernel(EvictArgs a, int vp
   const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
   const int32_t* tab = a.table + (int64_t)b * a.W;
   const int used = (r.n + (1 << a.psl) - 1) >> a.psl;  // pages of the sequence
-  const int32_t* cached = used <= MV_TAB ? sh_tab : nullptr;
-  if (cached != nullptr)
+  const int width = what < 0 ? 1 : vpr / slices, e0 = what < 0 ? 0 : (what % slices) * width;
+  pc_u32x4* const pool = (pc_u32x4*)(what < slices ? a.k_pages : a.v_pages);
+  if (used <= MV_TAB) {
     for (int i = threadIdx.x; i < used; i += MV_T) sh_tab[i] = tab[i];
-  __syncthreads();
-  if (what < 0) {
-    evict_move<float>(a.mass, a, kept, tab, cached, h, 1, 0, 1, r.n);
+    __syncthreads();
+    if (what < 0) evict_move<true>(a.mass, a, kept, tab, sh_tab, h, 1, e0, width, r.n);
+    else evict_move<true>(pool, a, kept, tab, sh_tab, h, vpr, e0, width, r.n);
   } else {
-    const int width = vpr / slices;
-    evict_move<pc_u32x4>((pc_u32x4*)(what < slices ? a.k_pages : a.v_pages), a, kept, tab, cached, h, vpr, (what % slices) * width, width, r.n);
+    if (what < 0) evict_move<false>(a.mass, a, kept, tab, sh_tab, h, 1, e0, width, r.n);
+    else evict_move<false>(pool, a, kept, tab, sh_tab, h, vpr, e0, width, r.n);
   }
 }
 
