@@ -209,6 +209,13 @@ __device__ constexpr int wa_key(int row) {
   return NV % 16 == 0 ? (row & 15) : NV % 8 == 0 ? (row & 7) : ((row >> 1) & 3);
 }
 
+// The same for the V rows of the bf16 kernel: its transposing reads take 32 bytes (two slots) of 8 rows at a time, so these rows must differ in the pair of
+// slots.  (With the key above a third of the LDS cycles were bank conflicts, now none are; the kernel's time is the same.)
+template <int NV>
+__device__ constexpr int wa_key_pairs(int row) {
+  return NV % 16 == 0 ? (row & 7) << 1 : NV % 8 == 0 ? (row >> 1 & 3) << 1 : (row >> 2 & 1) << 1;
+}
+
 // 16 bytes per lane from base + off to LDS address dst + 16 * lane (base and dst wave-uniform).  Not the builtin: the compiler takes any later LDS
 // read it cannot tell apart -- the transposing ones -- for a reader of what is in flight and waits for all of it, so that no tile is ever fetched ahead.
 // The waits for these loads are the kernels' own, ahead of the barrier that hands a tile over.
@@ -219,7 +226,7 @@ __device__ inline void wa_dma(const void* base, unsigned off, unsigned dst) {
 // Stages tiles of TK rows (NV 16-byte vectors each) of K or V into LDS, by the whole workgroup.  Rows past the sequence repeat its last one and
 // vectors past the head its first one: what they hold is never visible.  A lane's place in a tile is worked out once; a tile inside the sequence
 // then costs scalar arithmetic alone.  (Byte offsets inside a tile are 32-bit: row strides are below 2^24 elements, checked at the entry.)
-template <typename T, int TK, int NV>
+template <typename T, int TK, int NV, bool PAIRS = false>  // PAIRS: wa_key_pairs
 struct Stager {
   static constexpr int VE = 16 / (int)sizeof(T), N = TK * NV / 256;
   const T* base;
@@ -232,7 +239,7 @@ struct Stager {
   }
   __device__ int row(int i) const { return ((i * 4 + wu) * 64 + (int)(threadIdx.x & 63)) / NV; }
   __device__ int vec(int i, int dh) const {
-    const int v = (((i * 4 + wu) * 64 + (int)(threadIdx.x & 63)) % NV) ^ wa_key<NV>(row(i));
+    const int v = (((i * 4 + wu) * 64 + (int)(threadIdx.x & 63)) % NV) ^ (PAIRS ? wa_key_pairs<NV>(row(i)) : wa_key<NV>(row(i)));
     return v * VE < dh ? v : 0;
   }
   __device__ void operator()(int kt0, int dh, const unsigned char* dst) const {
@@ -303,7 +310,8 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
   const wa_bf16x8 ones = __builtin_bit_cast(wa_bf16x8, wa_s16x8{0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80});
   auto key0 = [&](int t) { return (t < ti.th ? t : ti.mf + (t - ti.th)) * TK; };
 
-  const Stager<bf16_t, TK, NV> stage_k(kb, a.k_row, len, dh, wu), stage_v(vb, a.v_row, len, dh, wu);
+  const Stager<bf16_t, TK, NV> stage_k(kb, a.k_row, len, dh, wu);
+  const Stager<bf16_t, TK, NV, true> stage_v(vb, a.v_row, len, dh, wu);
   stage_k(key0(0), dh, smem);
   stage_v(key0(0), dh, smem + HALF);
   // the queries are waited for here, once: a wait at their first use would stand inside the loop and take the tiles in flight with it
@@ -419,7 +427,7 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int key = j * 32 + g * 4 + (c >> 2);
-        const unsigned char* va = Vs + key * ROW + (((eb * 2 + ((c & 3) >> 1)) ^ wa_key<NV>(key)) << 4) + ((c & 1) << 3);
+        const unsigned char* va = Vs + key * ROW + (((eb * 2 + ((c & 3) >> 1)) ^ wa_key_pairs<NV>(key)) << 4) + ((c & 1) << 3);
         d[j][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va));
         d[j][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) wa_s16x4*)(va + 16 * ROW));  // the swizzle has a period of 16 rows
       }
