@@ -377,7 +377,7 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  * (valle/models/valle.py:1019-1033) is the case window = 0 of the first.
  *   row i of a sequence sees key j  iff  j < text_len  or  (j <= i and (window == 0 or i - j < window or j < sinks))
  * dtype VLE_DTYPE_F32 / _BF16 (T); head size a multiple of 8, <= 128; nhead a multiple of nhead_kv (query head h reads key-value head
- * h / (nhead / nhead_kv)), at most 256 per key-value head; strides in elements, every row and head on 16 bytes, rows less than 2^24 elements apart; scale > 0
+ * h / (nhead / nhead_kv)), at most 256 per key-value head; strides in elements, every row and head on 16 bytes, rows less than 2^24 elements apart; scale > 0, at most 2e38
  * (1 / sqrt(dh) as a rule).  All pointers DEVICE, index arrays int32.  A bad argument is refused with VLE_EINVAL before any launch;
  * what index arrays hold is bounded inside the kernels: offsets and lengths are clamped to the rows / the table, and a page id outside
  * [0, n_pages) is never followed -- its keys are absent.  The HIP device current at the call must be the stream's.
@@ -396,7 +396,7 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  *   keys with the largest mass (of equal ones the earlier; NaN counts as the largest), per key-value head, `budget` in all; text_len beyond the
  *   budget takes all of it, and what it leaves bounds `recent`.  The keys that stay move up in order, in place, with their mass.
  *   kept int32 [B][nhead_kv][budget]: their old positions, ascending (-1 past the end); new_lengths int32 [B] = min(lengths, budget).
- *   A page belongs to one sequence here. */
+ *   A page stands in the tables once here. */
 int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                             int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
                             const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,

@@ -163,3 +163,10 @@ def test_c_evict_refuses(kw):
 
 def test_nothing_to_do_is_no_error():
     assert _c_window(rows=0) == 0 and _c_decode(B=0) == 0 and _c_write(B=0, rows=0) == 0 and _c_evict(B=0) == 0
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.0e38])
+def test_c_scale_whose_base_2_form_overflows_is_refused(scale):
+    # scale * log2(e) would be infinite, and 0 * inf not a number, where the softmax of equal scores is their mean
+    assert _c_window(scale=scale) == _lib.VLE_EINVAL
+    assert _c_decode(scale=scale) == _lib.VLE_EINVAL and b"scale" in _lib.load().vle_last_error(None)

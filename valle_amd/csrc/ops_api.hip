@@ -320,7 +320,7 @@ extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, i
   if (const char* e = heads_fault(dtype, nhead, nhead_kv, dh)) return op_refuse(op, e);
   if (rows < 0 || rows > 0x7fff0000 || B < 0) return op_refuse(op, "bad number of rows or sequences");
   if (window < 0 || sinks < 0) return op_refuse(op, "window and sinks must not be negative");
-  if (!(scale > 0.f) || scale > 3.0e38f) return op_refuse(op, "scale must be positive and finite");
+  if (!(scale > 0.f) || scale > 2.0e38f) return op_refuse(op, "scale must be positive, at most 2e38");
   if (rows == 0) return VLE_OK;
   if (!q || !k || !v || !out || !seq_off_dev) return op_refuse(op, "null operand");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !vec_strides(dtype, q_row, q_head) ||
@@ -331,7 +331,7 @@ extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, i
   a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
   a.seq_off = seq_off_dev; a.text_len = text_len_dev; a.rows = rows; a.B = B; a.H = nhead; a.Hkv = nhead_kv; a.dh = dh;
   a.window = window; a.sinks = sinks; a.zero_rest = zero_rest;
-  a.sl2 = scale * 1.4426950408889634f;
+  a.sl2 = scale * 1.4426950408889634f;  // finite
   const int r = launch_window_attention((hipStream_t)stream, dtype, a);
   if (r == -1) return op_refuse(op, "too many rows times heads for one launch");
   return op_done(r, op);
@@ -379,7 +379,7 @@ extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void
   if (const char* e = heads_fault(dtype, nhead, nhead_kv, dh)) return op_refuse(op, e);
   if (const char* e = cache_fault(B, nhead_kv, dh, n_pages, table_width, page_size)) return op_refuse(op, e);
   if (window < 0 || sinks < 0) return op_refuse(op, "window and sinks must not be negative");
-  if (!(scale > 0.f) || scale > 3.0e38f) return op_refuse(op, "scale must be positive and finite");
+  if (!(scale > 0.f) || scale > 2.0e38f) return op_refuse(op, "scale must be positive, at most 2e38");
   if (B == 0) return VLE_OK;
   if (!q || !k_pages || !v_pages || !page_table_dev || !lengths_dev || !out) return op_refuse(op, "null operand");
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || !vec_strides(dtype, q_row, q_head))
@@ -395,7 +395,7 @@ extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void
   a.part_o = p.o_floats ? ws + p.score_floats : nullptr;
   a.part_ml = p.ml_floats ? ws + p.score_floats + p.o_floats : nullptr;
   a.Hkv = nhead_kv; a.G = nhead / nhead_kv; a.dh = dh; a.n_pages = n_pages; a.W = table_width; a.psl = log2_of(page_size);
-  a.window = window; a.sinks = sinks; a.sl2 = scale * 1.4426950408889634f;
+  a.window = window; a.sinks = sinks; a.sl2 = scale * 1.4426950408889634f;  // finite
   return op_done(launch_paged_decode((hipStream_t)stream, dtype, p, a, B), op);
 }
 

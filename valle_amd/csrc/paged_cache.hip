@@ -58,7 +58,8 @@ __device__ inline int split_tiles(int tt, int nsplit) { return nsplit == 1 ? max
 }  // namespace
 
 // ---- writing ---------------------------------------------------------------------------------------------------------------------
-// One wave per new token and per half (K, V): Hkv * dh elements in 16-byte vectors, contiguous reads, one dh-segment per head out.  HBM-bound copy.
+// One wave per new token and per half (K, V): Hkv * dh elements in 16-byte vectors, contiguous reads, one dh-segment per head out.
+// HBM-bound copy: 64 prompts of 150 - 420 rows, 16 heads of 64 (151 MB) 34 us = 4.4 TB/s, a plain copy reaches 4.9; one row for each of 6 sequences 3.0 us.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs a) {
   const int lane = threadIdx.x & 63;
@@ -109,6 +110,12 @@ int launch_paged_write(hipStream_t st, int dtype, const PagedWriteArgs& a) {
 // lane (g, c) loads dims c * DPL .. + DPL - 1 of its group's 8 keys (four whole rows per instruction) and one byte-permute per packed pair turns
 // them into the operands of DPL products, product j giving dims 4-lane-slot * DPL + j.  No LDS, no barrier in the loop; a group of one
 // head leaves 15 columns empty, which the matrix pipe has room for (it needs 1/16 of the time the HBM takes for the same keys).
+//
+// HBM-bound.  Measured: 3 sequences of 40k - 60k keys, 32 heads on 8 of 128, bf16 (684 MB): 110 us = 6.2 TB/s, and 4.7 the join; 16 sequences, window 1500
+// of 9k - 30k keys, 16 heads of 96, fp32 (312 MB): 60 us = 5.2 TB/s, and 4.7; 64 sequences of 330 - 1100 keys, 16 heads of 64, with mass (216 MB): 50 us = 4.3
+// TB/s, bound by the longest sequences, whose workgroups run on alone; one sequence of 1025 keys: 10.2 us, the steps' latency one after another.
+// A second tile of registers on its way was slower (138 -> 141 us and 73 -> 87 for the first two, at the time: fewer waves fit).
+
 // NT: past the memory-side cache
 template <bool NT, typename V>
 __device__ inline V pd_load(const void* p) {
@@ -452,7 +459,9 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
   // caches with 8 heads take 113 us, 43 (one third more than fit) 128, 64 (two rounds) 116, 128 (shorter parts, a longer join) 121.
   const int64_t slots = 256 * (dh <= 64 ? 5 : 3);
   p.nsplit = 1;
-  p.nw = groups < 512 && ng <= 8 ? 8 : 4;  // 8 waves: their outputs fit 32 KB of LDS for up to 8 heads
+  // 8 waves where groups are few (their outputs fit 32 KB of LDS for up to 8 heads): one sequence of 600 keys, 16 heads of 64, 6.9 us, with 4 waves 9.6;
+  // 16 sequences of 2000: 27 / 37; 24 of 1000: 24 / 23; 64 sequences: no difference
+  p.nw = groups < 512 && ng <= 8 ? 8 : 4;
   // One workgroup a head takes 7 us per 1000 keys of 64 (a CU alone pulls about 40 GB/s), the join costs 3 us and a launch on the host: one sequence of
   // 16 heads of 64 is faster unsplit up to 1040 keys (10.7 / 14.0 us a call), split from 1500 on (13.6 / 13.8; 13.8 / 10.0 in a graph).  A group for
   // every CU needs no split yet at 2000 keys (16 sequences, 16 heads: 27 / 31 us).
@@ -460,8 +469,10 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
     p.nw = 4;
     p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), std::max((int64_t)1, slots / groups));
   }
+  // past the memory-side cache where the keys do not fit: 684 MB 126 -> 115 us; 4 MB that would have stayed there: 10.6 -> 11.4
   p.stream = (int64_t)p.tiles * tk * B * Hkv * dh * (dtype == DT_F32 ? 8 : 4) > (int64_t)128 << 20;
-  // weights: by the workgroup that has all of a head's scores, where they fit beside its outputs; else by the join
+  // weights: by the workgroup that has all of a head's scores, where they fit beside its outputs; else by the join (64 sequences of 330 - 1100 keys,
+  // 16 heads: 50 us, by the join 56)
   p.score_lds = mass && p.nsplit == 1 && G <= 16 && (int64_t)p.tiles * tk * ng <= 7168 ? p.tiles * tk : 0;
   const bool join_mass = mass && p.score_lds == 0;
   p.ml_floats = (p.nsplit > 1 || join_mass) ? (size_t)(B * H * p.nsplit * 2) : 0;
@@ -505,6 +516,7 @@ int launch_paged_decode(hipStream_t st, int dtype, const PagedDecodePlan& p, Pag
 // Which keys stay: the first S and the last R of n, and of the n - S - R between them the M = budget - S - R with the most weight (of equal
 // weights the earlier).  One workgroup per (sequence, head) finds the M-th largest weight by three counting passes over its order-preserving
 // 32-bit key (11 + 11 + 10 bits, 2048 counters in LDS), then numbers the keys that stay in one more pass in the order of their positions.
+// Bound by the passes' latency: 4 sequences of 900 - 1500 keys, 16 heads: 8 us; 32 sequences of 4.5k - 9k keys, 8 heads: 21 us.
 constexpr int EV_T = 1024, EV_NW = EV_T / 64, EV_BINS = 2048;
 
 __device__ inline uint32_t ev_key(float m) {  // larger weight, larger key; NaN above everything, -0 = +0
@@ -756,14 +768,15 @@ int launch_kv_evict(hipStream_t st, int dtype, const EvictArgs& a, int B, int dh
   if (B <= 0) return 0;
   const int64_t most = (int64_t)a.W << a.psl;
   const dim3 sgrid(a.Hkv, B);
+  // candidates in registers where the table is short enough (4 sequences of 900 - 1500 keys, selection and move: 28 us, read again in every pass 30;
+  // 32 of 4.5k - 9k: 267 / 279)
   if (most <= 4 * EV_T) hipLaunchKernelGGL((kv_evict_select_kernel<4>), sgrid, dim3(EV_T), 0, st, a);
   else if (most <= 16 * EV_T) hipLaunchKernelGGL((kv_evict_select_kernel<16>), sgrid, dim3(EV_T), 0, st, a);
   else hipLaunchKernelGGL((kv_evict_select_kernel<0>), sgrid, dim3(EV_T), 0, st, a);
   const int vpr = dh * (dtype == DT_F32 ? 4 : 2) / 16;
-  // Slices of whole 128-byte lines; of 64 bytes where that leaves fewer than two workgroups a CU (measured with 256 threads: 4 sequences of 16 heads
-  // of 64: 40 -> 33 us; with 32 sequences of 8 heads of 128 half lines cost 295 -> 331 us)
-  int slices = vpr % 8 == 0 ? vpr / 8 : 1;
-  if (vpr % 4 == 0 && (int64_t)B * a.Hkv * 2 * slices < 512) slices = vpr / 4;
+  // Slices of whole 128-byte lines.  (Half lines: 32 sequences, 8 heads of 128, 267 -> 370 us; 4 sequences, 16 heads of 64, where that doubles the 128
+  // workgroups, 28 us both.)
+  const int slices = vpr % 8 == 0 ? vpr / 8 : 1;
   hipLaunchKernelGGL(kv_evict_move_kernel, dim3(a.Hkv, B, 2 * slices + 1), dim3(MV_T), 0, st, a, vpr, slices);
   return 0;
 }

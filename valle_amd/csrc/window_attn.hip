@@ -259,9 +259,14 @@ struct Stager {
 
 // ---- bf16 --------------------------------------------------------------------------------------------------------------------------
 // 4 waves, QW query fragments of 16 rows each; 64-key tiles of K and V go global -> LDS by DMA into one of two buffers while the other is
-// multiplied (a third buffer changed nothing); V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the matrix pipe (an all-ones
-// row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16 (8 bits: 2^-9 of each weight, which
-// averages out over the keys and stays below the output's own rounding).
+// multiplied (a third buffer changed nothing); V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the
+// matrix pipe (an all-ones row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16 (8 bits: 2^-9 of each weight,
+// which averages out over the keys and stays below the output's own rounding).
+//
+// Measured: one sequence of 12289 rows, 16 heads on 4 key-value heads of 128, window 2048: 220 us = 860 TFLOP/s of visible pairs, 71 % of what a large
+// library product reaches here (1206).  The matrix pipe is busy 40 % of the cycles, the vector pipe 30 % (exponentials, masks, conversions), LDS 20 %; two
+// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 91 us (238 MB; a copy of it takes 49): a wave of 16
+// rows computes 450 keys a row for 340 visible ones, and head size 64 has half the product per exponential.  Two short sequences: 5.0 us, less than a launch costs the host.
 template <int DHT, int QW>
 __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a) {
   constexpr int QB = 64 * QW, TK = 64, NV = DHT / 8, ROW = DHT * 2, KS = DHT / 32, EB = DHT / 16;
@@ -487,6 +492,8 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 // K feeds four products (contraction slot g of product u is dim 16 t + 4 g + u); V^T needs no transpose: product j of key r takes V[4 g + r][dim(c, j)],
 // with dim(c, j) the j-th of the up to 8 elements that lane c reads of a row.
 // NG = 2: two groups of 4 waves share the rows and take every other tile each; their halves are joined at the end.
+// Measured: two sequences of 700 - 1025 rows, 16 heads of 96, window 300: 57 us = 63 TFLOP/s of visible pairs (a large library product: 154); 1.75 workgroups
+// a CU, so that most wait for those with two, and tiles on the window's edges bound it.  One sequence of 4000 rows, 16 heads of 64, window 1000: 162 us = 88 TFLOP/s.
 template <int DHT, int NG>
 __global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArgs a) {
   constexpr int QB = 64, TK = 32, NV = DHT / 4, ROW = DHT * 4, KT = DHT / 16, DPL = DHT / 16;
@@ -675,10 +682,14 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   const bool f32 = dtype == DT_F32;
   // items of a head: the rows' runs, one more for every sequence's ragged last one, one for the rows of no sequence
   auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
-  const bool wide = !f32 && items(128) * a.H >= 1024;
+  // bf16, head size above 96, two workgroups a CU or more: 128 rows each, so that a fragment read from LDS feeds two products (32 heads of 128, sequences of
+  // 1000 rows: 1 of them 26.5 us with 64 rows / 32 with 128, 2: 42 / 38, 8: 125 / 116; 12289 rows, 16 heads: 705 / 579).  Smaller heads lose more by the
+  // registers than they win (16 sequences, 16 heads of 96: 91 / 98; 32 of 900, 16 heads of 64, window 256: 73 / 80, no window 107 / 119).
+  const bool wide = !f32 && a.dh > 96 && items(128) * a.H >= 512;
   const int64_t n = items(wide ? 128 : 64) * a.H;
   // fp32, at most about one workgroup a CU: a second group of waves halves each one's walk (one sequence of 1025 rows, 16 heads of 64: 66 -> 58 us;
-  // 4 key-value heads of 128, window 300: 51 -> 40).  With more, the tiles of both groups keep a second workgroup off the CU (window_fp32 57 -> 65 us).
+  // 4 key-value heads of 128, window 300: 51 -> 40).  With more, the tiles of both groups keep a second workgroup off the CU (two sequences of 700 - 1025 rows,
+  // 16 heads of 96, window 300: 57 -> 65 us; 16-key tiles, which leave room for it, are slower from 300 rows to 16 sequences: 58 / 61, 302 / 336).
   const bool pair = f32 && n <= 384;
   if (n > 0xffffff) return -1;  // 2^32 work items
   const dim3 grid((unsigned)n), block(256);
@@ -686,7 +697,7 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   do {                                                                                          \
     if (pair) hipLaunchKernelGGL((window_attn_f32_kernel<DHT, 2>), grid, dim3(512), 0, st, a);   \
     else if (f32) hipLaunchKernelGGL((window_attn_f32_kernel<DHT, 1>), grid, block, 0, st, a);   \
-    else if (wide) hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 2>), grid, block, 0, st, a); \
+    else if (wide) hipLaunchKernelGGL((window_attn_bf16_kernel<128, 2>), grid, block, 0, st, a); \
     else hipLaunchKernelGGL((window_attn_bf16_kernel<DHT, 1>), grid, block, 0, st, a);          \
   } while (0)
   if (a.dh <= 32) VLE_WA(32);

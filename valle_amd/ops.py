@@ -575,7 +575,7 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     equal ones the earlier; NaN counts as the largest), `budget` in all, for every key-value head by itself; a text longer than the budget takes all of
     it, and what it leaves bounds `recent`.  They move up in the order they had, with their mass.  Returns (kept int32 (B, Hkv, budget): the old
     positions, ascending, -1 past the end; lengths int32 (B,) = min(lengths, budget)): the pages behind the new lengths are free.
-    A page must belong to one sequence alone here."""
+    A page must stand in the tables once, at one place of one sequence."""
     who = "kv_evict"
     if mass is None:
         _refuse(who, "mass is needed")
