@@ -231,6 +231,20 @@ __device__ inline float wave_max_dpp(float v) {
   return fmaxf(fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)), fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
 }
 
+template <int CTRL, int ROWS>
+__device__ inline int dpp_or0_i32(int v) {  // 0 where the lane has no source, or its row is not in ROWS
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ inline int wave_scan_i(int v) {  // inclusive prefix sum over the lanes
+  v += dpp_or0_i32<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v += dpp_or0_i32<0x112, 0xf>(v);
+  v += dpp_or0_i32<0x114, 0xf>(v);
+  v += dpp_or0_i32<0x118, 0xf>(v);
+  v += dpp_or0_i32<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+  v += dpp_or0_i32<0x143, 0xc>(v);
+  return v;
+}
+
 // Block-wide sum for blockDim.x == NW*64; `red` is NW floats of LDS; all threads get the result.
 template <int NW>
 __device__ inline float block_sum(float v, float* red) {

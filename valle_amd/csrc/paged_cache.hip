@@ -585,12 +585,7 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
     __syncthreads();
     // thread t counts bins 2047 - 2 t and 2046 - 2 t: an inclusive scan from the top finds the bin the need-th largest falls into
     const int hi = bin[EV_BINS - 1 - 2 * tid], lo = bin[EV_BINS - 2 - 2 * tid];
-    int inc = hi + lo;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += t;
-    }
+    const int inc = wave_scan_i(hi + lo);
     if (lane == 63) wsum[w] = inc;
     __syncthreads();
     int before = inc - hi - lo;
@@ -633,13 +628,7 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
         v[i] = lane * PER + i < KPT * EV_NW ? cnt[w][lane * PER + i] : 0;
         sum += v[i];
       }
-      int inc = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += t;
-      }
-      inc -= sum;
+      int inc = wave_scan_i(sum) - sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         if (lane * PER + i < KPT * EV_NW) cnt[w][lane * PER + i] = inc;

@@ -49,20 +49,12 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
     off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
     return (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
   };
-  auto scan = [&](int x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(x, o, 64);
-      if (lane >= o) x += t;
-    }
-    return x;
-  };
   int lo = 0, hi = a.B;
   const int per = (a.B + 63) >> 6;
   if (per > 1) {  // many sequences: which lane's share of them holds the item
     int sum = 0, off;
     for (int b = lane * per; b < min((lane + 1) * per, a.B); ++b) sum += (rows_of(b, off) + QB - 1) / QB;
-    const int inc = scan(sum);
+    const int inc = wave_scan_i(sum);
     const unsigned long long past = __ballot(at < inc);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -81,7 +73,7 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
       if (a.text_len) text = a.text_len[b];  // (with the offsets, not a round trip to memory later)
       len = rows_of(b, off);
     }
-    const int inc = scan((len + QB - 1) / QB);
+    const int inc = wave_scan_i((len + QB - 1) / QB);
     const unsigned long long past = __ballot(at < inc);
     if (past) {
       const int l = __builtin_ctzll(past);
@@ -121,8 +113,6 @@ struct Sight {
   int hd, lo, i;
   // (& and | on purpose: a select per key, no branches)
   __device__ bool sees(int j) const { return (j < hd) | ((j >= lo) & (j <= i)); }
-  __device__ bool all(int j0, int n) const { return (j0 + n <= hd) | ((j0 >= lo) & (j0 + n - 1 <= i)); }
-  __device__ bool any(int j0, int n) const { return (j0 < hd) | ((j0 <= i) & (j0 + n - 1 >= lo)); }
 };
 __device__ inline Sight sight_of(int i, int text, int window, int sinks) {
   Sight s;
@@ -130,6 +120,16 @@ __device__ inline Sight sight_of(int i, int text, int window, int sinks) {
   s.lo = window > 0 ? max(0, i - window + 1) : 0;
   s.i = i;
   return s;
+}
+
+// What the rows i0 .. i1 of a wave see of the keys j0 .. j0 + n - 1 (both ends of a row's sight grow with the row): scalar arithmetic.
+struct Sights {
+  Sight first, last;
+  __device__ bool all(int j0, int n) const { return j0 + n <= first.hd || (j0 >= last.lo && j0 + n - 1 <= first.i); }
+  __device__ bool none(int j0, int n) const { return j0 >= last.hd && (j0 > last.i || j0 + n - 1 < first.lo); }
+};
+__device__ inline Sights sights_of(int i0, int i1, int text, int window, int sinks) {
+  return Sights{sight_of(i0, text, window, sinks), sight_of(i1, text, window, sinks)};
 }
 
 // One row over its visible keys alone, by one wave: 64 keys at a time, a lane the score of one, then two elements of the output as the average so far.
@@ -265,8 +265,8 @@ struct Stager {
 //
 // Measured: one sequence of 12289 rows, 16 heads on 4 key-value heads of 128, window 2048: 220 us = 860 TFLOP/s of visible pairs, 71 % of what a large
 // library product reaches here (1206).  The matrix pipe is busy 40 % of the cycles, the vector pipe 30 % (exponentials, masks, conversions), LDS 20 %; two
-// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 91 us (238 MB; a copy of it takes 49): a wave of 16
-// rows computes 450 keys a row for 340 visible ones, and head size 64 has half the product per exponential.  Two short sequences: 5.0 us, less than a launch costs the host.
+// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 94 us (238 MB; a copy of it takes 49): the vector pipe
+// bounds it -- a wave of 16 rows computes 460 keys a row for 340 visible ones, and head size 64 has half the product per exponential.  Two short sequences: 5.0 us, less than a launch costs the host.
 template <int DHT, int QW>
 __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a) {
   constexpr int QB = 64 * QW, TK = 64, NV = DHT / 8, ROW = DHT * 2, KS = DHT / 32, EB = DHT / 16;
@@ -286,6 +286,7 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
   const bf16_t* vb = (const bf16_t*)a.v + (int64_t)pl.off * a.v_row + (int64_t)hk * a.v_head;
 
   Sight see[QW];
+  Sights group[QW];  // of the fragment's 16 rows
   bool valid[QW];
   wa_bf16x8 qf[QW][KS];
 #pragma unroll
@@ -293,6 +294,8 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
     const int i = q0 + (w * QW + f) * 16 + c;
     valid[f] = i < len;
     see[f] = sight_of(min(i, len - 1), text, a.window, a.sinks);
+    const int i0 = q0 + (wu * QW + f) * 16;
+    group[f] = sights_of(min(i0, len - 1), min(i0 + 15, len - 1), text, a.window, a.sinks);
     const bf16_t* qp = (const bf16_t*)a.q + (int64_t)(pl.off + min(i, len - 1)) * a.q_row + (int64_t)pl.h * a.q_head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -335,14 +338,14 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
       stage_k(key0(t + 1), dh, nb);
       stage_v(key0(t + 1), dh, nb + HALF);
     }
-    bool some = false, all = true;
+    bool none = true, unmasked = true;
 #pragma unroll
     for (int f = 0; f < QW; ++f) {
-      some |= see[f].any(kt0, TK);
-      all &= see[f].all(kt0, TK);
+      none = none && group[f].none(kt0, TK);
+      unmasked = unmasked && group[f].all(kt0, TK);
     }
-    if (!__any(some)) continue;
-    const bool unmasked = __all(all);  // a masked tile's key that is not finite makes the row NaN: computed again at the end
+    if (none) continue;
+    // (a masked tile's key that is not finite makes the row NaN: computed again at the end)
 
     // ---- S^T = K Q^T: the accumulators start from the mask (0 or -inf) ----
     wa_f32x4 s[QW][4];
@@ -375,6 +378,7 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 #pragma unroll
       for (int f = 0; f < QW; ++f) {
         // key number 16 kb4 + r of this lane is visible from lo to hi, or, in a tile of the head, below hd: compares with constants, as few as the tile needs
+        // (a branch for every 16 keys, most of which are visible or hidden as a whole, is slower: 73 -> 86 us for 32 sequences of 900 rows, heads of 64)
         const int hi = see[f].i - kt0 - g * 4, lo = see[f].lo - kt0 - g * 4, hd = see[f].hd - kt0 - g * 4;
         auto mask = [&](auto hidden) {
 #pragma unroll
@@ -383,8 +387,8 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
             for (int r = 0; r < 4; ++r) s[f][kb4][r] = hidden(kb4 * 16 + r) ? -INFINITY : 0.f;
         };
         if (t < ti.th) mask([=](int k) { return (k >= hd) & ((k < lo) | (k > hi)); });
-        else if (!__any(lo > -g * 4)) mask([=](int k) { return k > hi; });
-        else if (!__any(hi < TK - 1 - g * 4)) mask([=](int k) { return k < lo; });
+        else if (group[f].last.lo <= kt0) mask([=](int k) { return k > hi; });
+        else if (group[f].first.i >= kt0 + TK - 1) mask([=](int k) { return k < lo; });
         else mask([=](int k) { return (k < lo) | (k > hi); });
       }
       scores();
@@ -517,6 +521,7 @@ __global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArg
   const int i = q0 + w * 16 + c;
   const bool valid = i < len;
   const Sight see = sight_of(min(i, len - 1), text, a.window, a.sinks);
+  const Sights rows = sights_of(min(q0 + w * 16, len - 1), min(q0 + w * 16 + 15, len - 1), text, a.window, a.sinks);
   wa_f32x4 qf[KT];
   const float* qp = (const float*)a.q + (int64_t)(pl.off + min(i, len - 1)) * a.q_row + (int64_t)pl.h * a.q_head;
 #pragma unroll
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArg
     }
     if (t >= ti.tt) continue;
     const int kt0 = key0(t);
-    if (!__any(see.any(kt0, TK))) continue;
+    if (rows.none(kt0, TK)) continue;
     wa_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     wa_f32x4 ka[2][2];  // [buffer][16-key tile]: the next 16 dims' fragments are read while these are multiplied
     auto read_k = [&](wa_f32x4 (&d)[2], int t4) {
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArg
         for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[t4 & 1][kt][u], qf[t4][u], s[kt], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const bool unmasked = __all(see.all(kt0, TK));
+    const bool unmasked = rows.all(kt0, TK);
     float mt = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
