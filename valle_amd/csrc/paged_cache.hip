@@ -114,7 +114,8 @@ int launch_paged_write(hipStream_t st, int dtype, const PagedWriteArgs& a) {
 // HBM-bound.  Measured: 3 sequences of 40k - 60k keys, 32 heads on 8 of 128, bf16 (684 MB): 110 us = 6.2 TB/s, and 4.7 the join; 16 sequences, window 1500
 // of 9k - 30k keys, 16 heads of 96, fp32 (312 MB): 60 us = 5.2 TB/s, and 4.7; 64 sequences of 330 - 1100 keys, 16 heads of 64, with mass (216 MB): 50 us = 4.3
 // TB/s, bound by the longest sequences, whose workgroups run on alone; one sequence of 1025 keys: 10.2 us, the steps' latency one after another.
-// A second tile of registers on its way was slower (138 -> 141 us and 73 -> 87 for the first two, at the time: fewer waves fit).
+// A second tile of registers on its way is slower, also where workgroups are few (138 -> 141 us and 73 -> 87 for the first two, at the time; 10.2 -> 10.6
+// for the last).
 
 // NT: past the memory-side cache
 template <bool NT, typename V>
