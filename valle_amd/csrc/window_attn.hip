@@ -264,9 +264,10 @@ struct Stager {
 // which averages out over the keys and stays below the output's own rounding).
 //
 // Measured: one sequence of 12289 rows, 16 heads on 4 key-value heads of 128, window 2048: 220 us = 860 TFLOP/s of visible pairs, 71 % of what a large
-// library product reaches here (1206).  The matrix pipe is busy 40 % of the cycles, the vector pipe 30 % (exponentials, masks, conversions), LDS 20 %; two
-// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 94 us (238 MB; a copy of it takes 49): the vector pipe
-// bounds it -- a wave of 16 rows computes 460 keys a row for 340 visible ones, and head size 64 has half the product per exponential.  Two short sequences: 5.0 us, less than a launch costs the host.
+// library product reaches here (1206).  The matrix pipe is busy 41 % of the cycles, the vector pipe 39 % (exponentials, masks, conversions), LDS 20 %; two
+// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 94 us (238 MB; a copy of it takes 49): vector pipe
+// 51 %, matrix pipe 21 %, the rest waits -- a wave of 16 rows computes 460 keys a row for 340 visible ones, head size 64 has half the product per
+// exponential, and walks of 8 tiles do not hide their start.  Two short sequences: 5.0 us, less than a launch costs the host.
 template <int DHT, int QW>
 __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a) {
   constexpr int QB = 64 * QW, TK = 64, NV = DHT / 8, ROW = DHT * 2, KS = DHT / 32, EB = DHT / 16;
