@@ -216,6 +216,38 @@ def test_window_attention_long(dtype, rows, H, Hkv, dh, window, sinks, text):
         near(got[::97, h], want.cpu(), tol.cpu(), f"head {h}")
 
 
+@pytest.mark.parametrize("dh,Hkv,window,sinks", [(128, 4, 33, 2), (120, 32, 150, 0), (104, 1, 0, 0), (96, 4, 70, 3)])
+def test_window_attention_many_ragged_sequences_of_large_heads(dh, Hkv, window, sinks):
+    """Work enough for the largest items, and sequences that end inside them; rows of no sequence; a key that is not a number reaches only the rows that see it."""
+    g, H, dtype = gen(dh), 32, torch.bfloat16
+    lens = [0, 1, 15, 16, 17, 127, 128, 129, 0, 200, 255, 256, 257, 63, 64, 65, 300]
+    text = [0, 1, 3, 0, 17, 40, 0, 64, 0, 0, 65, 0, 9, 70, 0, 0, 120]
+    off = offsets(lens)
+    rows = off[-1] + 13
+    q, k, v = rnd(g, rows, H, dh, dtype=dtype), rnd(g, rows, Hkv, dh, dtype=dtype), rnd(g, rows, Hkv, dh, dtype=dtype)
+    poisoned = {9: 180, 16: 130}  # sequence: key
+    for b, j in poisoned.items():
+        k[off[b] + j] = float("nan")
+    q, k, v = q.to(DEV), k.to(DEV), v.to(DEV)
+    got = ops.window_attention(q, k, v, i32(off), window=window, sinks=sinks, text_len=i32(text))
+    assert bool((got[off[-1]:] == 0).all())
+    u = half_step(dtype)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        r = slice(off[b], off[b + 1])
+        m = torch.stack([sees(n, i, min(text[b], n), window, sinks) for i in range(n)]).to(DEV)
+        hit = m[:, poisoned[b]] if b in poisoned else torch.zeros(n, dtype=torch.bool, device=DEV)
+        assert bool(got[r][hit].isnan().all())
+        for h in range(H):
+            qh, kh, vh = q[r, h].double(), k[r, h // (H // Hkv)].double().nan_to_num(0.0), v[r, h // (H // Hkv)].double()
+            spread = float((qh.abs() @ kh.abs().T).max()) / math.sqrt(dh)
+            w = torch.softmax(((qh @ kh.T) / math.sqrt(dh)).masked_fill(~m, -math.inf), 1)
+            want, delta = w @ vh, 2 * (dh + 4) * 2.0 ** -24 * spread + 2.0 ** -20
+            tol = (2 * (delta + n * 2.0 ** -24) + 2 * u) * (w @ vh.abs()) + u * want.abs()
+            near(got[r, h][~hit], want[~hit].cpu(), tol[~hit].cpu(), f"sequence {b} head {h}")
+
+
 def test_window_attention_is_the_prefix_lm_attention_without_a_window():
     """window = 0 and one key-value head per query head: the mask of ops.attention (both bf16: weights and result rounded)."""
     g, H, dh, lens, text = gen(8), 4, 64, [90, 70], [20, 31]
