@@ -248,6 +248,22 @@ def test_window_attention_many_ragged_sequences_of_large_heads(dh, Hkv, window, 
             near(got[r, h][~hit], want[~hit].cpu(), tol[~hit].cpu(), f"sequence {b} head {h}")
 
 
+def test_window_attention_offsets_whose_runs_overflow_their_count():
+    """Offsets that go back and forth: 2^31 runs of rows and more, of which the launch has work items for a few.  Nothing outside `out` is written, and inside it
+    only averages."""
+    H, dh, B = 1024, 8, 5800
+    rows = 64 * B
+    assert (B // 2) * B * (H // 8) > 2 ** 31
+    q = torch.zeros(rows, H, dh, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(rows, 4, dh, dtype=torch.bfloat16, device=DEV)
+    room = torch.full(((rows + 256) * H * dh,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = room[128 * H * dh: -128 * H * dh].view(rows, H, dh)
+    ops.window_attention(q, k, k + 1, i32([0, rows] * (B // 2) + [0]), window=1, out=out)
+    torch.cuda.synchronize()
+    assert bool((room[: 128 * H * dh] == 7).all()) and bool((room[-128 * H * dh:] == 7).all())
+    assert bool(((out == 1) | (out == 7)).all())
+
+
 def test_window_attention_is_the_prefix_lm_attention_without_a_window():
     """window = 0 and one key-value head per query head: the mask of ops.attention (both bf16: weights and result rounded)."""
     g, H, dh, lens, text = gen(8), 4, 64, [90, 70], [20, 31]

@@ -29,9 +29,10 @@ typedef unsigned wa_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float WA_DEFER = 8.f;  // exp2-domain growth of a row's maximum below which its reference stays (weights up to 2^8)
 
-// Where a workgroup works: sequence, head, first query row.  Work items are numbered head by head, a sequence's row runs one after another
-// (late ones, which see most without a window, first), so that neighbours read the same keys; `seq` = -1: no sequence is left for this item and
-// `rest` counts the items past the last one.
+// Where a workgroup works: sequence, head, first query row.  Work items are numbered group of heads by group (what one XCD holds of them, where 8 divides
+// their number), sequence by sequence, run of rows by run (late ones, which see most without a window, first), head by head: neighbours read the same keys,
+// and work shrinks from item to item (head by head instead: one sequence of 4000 rows without a window, 16 heads of 64, bf16 51 -> 66 us, fp32 303 -> 430).
+// `seq` = -1: no sequence is left for this item and `rest` counts the runs of its head past the last one.
 struct Place {
   int h, seq, off, len, text, q0, rest;
 };
@@ -40,11 +41,14 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
   const int lane = threadIdx.x & 63;
   const int per_head = gridDim.x / a.H;
   // workgroup L runs on XCD L % 8, each with its own L2: every XCD gets a contiguous run of the items
-  const int nb = gridDim.x, q = nb / 8, rem = nb % 8, xcd = blockIdx.x % 8, idx = blockIdx.x / 8;
+  const int nb = gridDim.x, q = nb / 8, rem = nb % 8, xcd = blockIdx.x % 8;
+  int idx = blockIdx.x / 8;
+  // ... and deals them out to its 32 CUs in turn: every other round backwards, so that the CUs with the longest item of one get the shortest of the next
+  if ((idx & 32) && (idx | 31) < q + (xcd < rem)) idx ^= 31;
   const int item = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + idx;
+  const int hg = a.H % 8 == 0 ? a.H / 8 : 1, group = item / (per_head * hg);
   Place p;
-  p.h = item / per_head;
-  int at = item - p.h * per_head;
+  int at = item - group * per_head * hg;
   auto rows_of = [&](int b, int& off) {  // clamped to the rows there are, whatever the offsets say
     off = (int)min((int64_t)max(a.seq_off[b], 0), a.rows);
     return (int)min((int64_t)max(a.seq_off[b + 1], off), a.rows) - off;
@@ -53,7 +57,7 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
   const int per = (a.B + 63) >> 6;
   if (per > 1) {  // many sequences: which lane's share of them holds the item
     int sum = 0, off;
-    for (int b = lane * per; b < min((lane + 1) * per, a.B); ++b) sum += (rows_of(b, off) + QB - 1) / QB;
+    for (int b = lane * per; b < min((lane + 1) * per, a.B); ++b) sum += (rows_of(b, off) + QB - 1) / QB * hg;
     const int inc = wave_scan_i(sum);
     const unsigned long long past = __ballot(at < inc);
     if (past) {
@@ -73,23 +77,26 @@ __device__ inline Place place_of(const WindowAttnArgs& a) {
       if (a.text_len) text = a.text_len[b];  // (with the offsets, not a round trip to memory later)
       len = rows_of(b, off);
     }
-    const int inc = wave_scan_i((len + QB - 1) / QB);
+    const int inc = wave_scan_i((len + QB - 1) / QB * hg);
     const unsigned long long past = __ballot(at < inc);
     if (past) {
       const int l = __builtin_ctzll(past);
-      p.seq = b0 + l;
       p.off = __builtin_amdgcn_readlane(off, l);
       p.len = __builtin_amdgcn_readlane(len, l);
       p.text = min(max(__builtin_amdgcn_readlane(text, l), 0), p.len);
-      p.q0 = (__builtin_amdgcn_readlane(inc, l) - 1 - at) * QB;
-      p.rest = 0;
+      const int left = __builtin_amdgcn_readlane(inc, l) - 1 - at, run = left / hg;
+      p.h = group * hg + (left >= 0 ? left - run * hg : 0);
+      p.q0 = run * QB;
+      p.rest = 0x7fffffff;
+      p.seq = (left >= 0) & (run < (p.len + QB - 1) / QB) ? b0 + l : -1;  // -1: offsets that go back and forth until the count of their runs overflows
       return p;
     }
     at -= __builtin_amdgcn_readlane(inc, 63);
   }
   p.seq = -1;
   p.off = p.len = p.text = p.q0 = 0;
-  p.rest = at;
+  p.rest = at < 0 ? 0x7fffffff : at / hg;  // (< 0: the same)
+  p.h = group * hg + (at < 0 ? 0 : at % hg);
   return p;
 }
 
@@ -505,7 +512,10 @@ __global__ __launch_bounds__(256 * NG) void window_attn_f32_kernel(WindowAttnArg
   constexpr int HALF = TK * ROW, BUF = 2 * HALF;
   constexpr int A4 = DPL >= 4 ? 4 : 2;           // elements of a lane's first chunk of a V row, and of its second
   constexpr int B4 = DPL - A4;                   // (DHT 32: 2, 64: 4, 96: 4 + 2, 128: 4 + 4)
-  __shared__ __attribute__((aligned(16))) unsigned char smem[2 * NG * BUF];
+  // two groups: more than half of the LDS, so that a CU takes one workgroup at a time and the next goes to the first that is free (one sequence of 1300 rows,
+  // 16 heads of 64: 70 -> 62 us)
+  constexpr int LDS = NG == 2 && 2 * NG * BUF < (82 << 10) ? 82 << 10 : 2 * NG * BUF;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[LDS];
   const Place pl = place_of<QB>(a);
   if (pl.seq < 0) {
     if (a.zero_rest) zero_rows<float, QB>(a, pl.h, pl.rest);
@@ -689,14 +699,15 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   // items of a head: the rows' runs, one more for every sequence's ragged last one, one for the rows of no sequence
   auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
   // bf16, head size above 96, two workgroups a CU or more: 128 rows each, so that a fragment read from LDS feeds two products (32 heads of 128, sequences of
-  // 1000 rows: 1 of them 26.5 us with 64 rows / 32 with 128, 2: 42 / 38, 8: 125 / 116; 12289 rows, 16 heads: 705 / 579).  Smaller heads lose more by the
+  // 1000 rows: 1 of them 26.5 us with 64 rows / 32 with 128, 2: 42 / 38, 8: 125 / 116; 12289 rows, 16 heads: 705 / 579; all before the items' present order).  Smaller heads lose more by the
   // registers than they win (16 sequences, 16 heads of 96: 91 / 98; 32 of 900, 16 heads of 64, window 256: 73 / 80, no window 107 / 119).
   const bool wide = !f32 && a.dh > 96 && items(128) * a.H >= 512;
   const int64_t n = items(wide ? 128 : 64) * a.H;
-  // fp32, at most about one workgroup a CU: a second group of waves halves each one's walk (one sequence of 1025 rows, 16 heads of 64: 66 -> 58 us;
-  // 4 key-value heads of 128, window 300: 51 -> 40).  With more, the tiles of both groups keep a second workgroup off the CU (two sequences of 700 - 1025 rows,
-  // 16 heads of 96, window 300: 57 -> 65 us; 16-key tiles, which leave room for it, are slower from 300 rows to 16 sequences: 58 / 61, 302 / 336).
-  const bool pair = f32 && n <= 384;
+  // fp32, about one workgroup a CU (without a window, where the late rows' work is the longest and goes first, up to one and a half): a second group of waves
+  // halves each one's walk.  One sequence, 16 heads of 96, no window: 1300 rows 103 -> 80 us, 1600 131 -> 97, but 2000 141 -> 167; window 256: 1024 rows
+  // 28 -> 27, but 1300 42 -> 48, where a second workgroup a CU is worth more.  (16-key tiles, which leave room for it, are slower from 300 rows to 16 sequences:
+  // 58 / 61, 302 / 336.)
+  const bool pair = f32 && n <= (a.window > 0 ? 320 : 448);
   if (n > 0xffffff) return -1;  // 2^32 work items
   const dim3 grid((unsigned)n), block(256);
 #define VLE_WA(DHT)                                                                             \
