@@ -405,25 +405,27 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
     wa_bf16x8 pf[QW][2];
 #pragma unroll
     for (int f = 0; f < QW; ++f) {
-      // s sl2 - M in one fma: what the rounding of M leaves is a factor of the whole row and cancels, up to scores of 2^31, where it passes the
-      // exponent's range and the row is computed again
-      const float nm = M[f] == -INFINITY ? 0.f : -M[f];
+      // s sl2 - M in one fma, of every tile against M as it is stored: the same rounding of M for the whole row, which cancels, so that equal scores get equal
+      // weights whatever their size -- up to scores of 2^31, where it passes the exponent's range and the row is computed again
+      wa_f32x4 x[4];
+      auto relative = [&](float ref) {
 #pragma unroll
-      for (int kb4 = 0; kb4 < 4; ++kb4)
+        for (int kb4 = 0; kb4 < 4; ++kb4)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[f][kb4][r] = fmaf(s[f][kb4][r], sl2, nm);
-      float mt = fmaxf(fmaxf(s[f][0][0], s[f][0][1]), fmaxf(s[f][0][2], s[f][0][3]));
+          for (int r = 0; r < 4; ++r) x[kb4][r] = fmaf(s[f][kb4][r], sl2, ref == -INFINITY ? 0.f : -ref);
+      };
+      relative(M[f]);
+      float mt = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
 #pragma unroll
-      for (int kb4 = 1; kb4 < 4; ++kb4) mt = fmaxf(mt, fmaxf(fmaxf(s[f][kb4][0], s[f][kb4][1]), fmaxf(s[f][kb4][2], s[f][kb4][3])));
+      for (int kb4 = 1; kb4 < 4; ++kb4) mt = fmaxf(mt, fmaxf(fmaxf(x[kb4][0], x[kb4][1]), fmaxf(x[kb4][2], x[kb4][3])));
       // the reference stays while no score exceeds it by more than WA_DEFER: the result does not depend on it, O and the sum carry the same factor
       if (!__all((mt <= WA_DEFER) & (M[f] != -INFINITY))) {
         mt = rows4_max(mt);
         const bool begun = M[f] != -INFINITY;
-        const float d = begun ? fmaxf(mt, 0.f) : (mt == -INFINITY ? 0.f : mt);
-        const float alpha = begun ? __builtin_amdgcn_exp2f(-d) : 1.f;
-        M[f] = begun ? M[f] + d : mt;
-#pragma unroll
-        for (int kb4 = 0; kb4 < 4; ++kb4) s[f][kb4] -= d;
+        const float was = M[f];
+        M[f] = begun ? was + fmaxf(mt, 0.f) : mt;
+        const float alpha = begun ? __builtin_amdgcn_exp2f(was - M[f]) : 1.f;  // from the two as stored; a rounding of the difference is 2^-24 of it, of a weight 2^-difference
+        relative(M[f]);  // not x less the step: x is rounded at the old reference's distance
         ol[f] *= alpha;
 #pragma unroll
         for (int eb = 0; eb < EB; ++eb) o[f][eb] *= alpha;
@@ -431,11 +433,11 @@ __global__ __launch_bounds__(256) void window_attn_bf16_kernel(WindowAttnArgs a)
 #pragma unroll
       for (int kb4 = 0; kb4 < 4; ++kb4)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[f][kb4][r] = __builtin_amdgcn_exp2f(s[f][kb4][r]);
+        for (int r = 0; r < 4; ++r) x[kb4][r] = __builtin_amdgcn_exp2f(x[kb4][r]);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int tt = 0; tt < 8; ++tt) pf[f][j][tt] = (__bf16)s[f][2 * j + (tt >> 2)][tt & 3];
+        for (int tt = 0; tt < 8; ++tt) pf[f][j][tt] = (__bf16)x[2 * j + (tt >> 2)][tt & 3];
     }
     // ---- O^T += V^T P^T ----
     // the transposing read hands lane c the elements V[k0 .. k0 + 3][16 eb + c] of the rows whose addresses lanes c / 4 supply
