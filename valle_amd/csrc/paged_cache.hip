@@ -139,7 +139,65 @@ __device__ inline void pd_load_words(unsigned (&dst)[N], const void* src) {  // 
   }
 }
 
-template <typename T, int DHT, int NW, bool WHOLE, bool NT>  // WHOLE: dh == DHT, no lane is ever outside the head
+// Element e of one head's output once more, by one wave (an element a lane): the running average of the visible values instead of their sum over a denominator.
+// For results that are not finite, a rarity: a sum past the largest number, whose average need not be, and infinities, which the two parts of a bf16 weight
+// (one of them may be negative) turn into NaN.  64 keys at a time, a lane the score of one; 8 values on their way.
+// Done early where every element that is asked for is NaN already.
+template <typename T, int TK>
+__device__ inline float pd_exact(const PagedDecodeArgs& a, const Span<TK>& sp, int b, int h, int e, bool asked) {
+#pragma clang fp contract(off)  // as for the scores of the kernel below
+  constexpr int VE = Elem<T>::VEC;
+  const int lane = threadIdx.x & 63, kvh = h / a.G, ps = 1 << a.psl;
+  const int64_t page_elems = (int64_t)a.Hkv * ps * a.dh;
+  const T* q = (const T*)a.q + (int64_t)b * a.q_b + (int64_t)h * a.q_h;
+  const T* kbase = (const T*)a.k_pages + (int64_t)kvh * ps * a.dh;
+  const T* vbase = (const T*)a.v_pages + (int64_t)kvh * ps * a.dh;
+  e = min(e, a.dh - 1);
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int i0 = 0; i0 < sp.tt * TK; i0 += 64) {
+    const int i = i0 + lane, j = sp.key0(i / TK) + i % TK;
+    const bool in = (i < sp.tt * TK) & sp.sees(j);
+    const int id = in ? a.table[(int64_t)b * a.W + (j >> a.psl)] : -1;
+    const bool vis = (unsigned)id < (unsigned)a.n_pages;
+    const int page = vis ? id : 0, at = vis ? (j & (ps - 1)) * a.dh : 0;  // what is not visible is not looked at: its loads go to the pool's first key
+    if (!__any(vis)) continue;
+    float s = -INFINITY;
+    if (vis) {
+      float sum = 0.f;
+      for (int d = 0; d < a.dh; d += VE) {
+        float x[VE], y[VE];
+        load_vec16(q + d, x);
+        load_vec16(kbase + (int64_t)page * page_elems + at + d, y);
+#pragma unroll
+        for (int u = 0; u < VE; ++u) sum = fmaf(x[u], y[u], sum);
+      }
+      s = sum * a.sl2;
+    }
+    if (__any(s != s)) return __builtin_nanf("");
+    const float mn = fmaxf(m, wave_max(s)), ref = mn == -INFINITY ? 0.f : mn;
+    const float p = __builtin_amdgcn_exp2f(s - ref), was = l * __builtin_amdgcn_exp2f(m - ref), now = was + wave_sum(p);
+    m = mn;
+    l = now;
+    if (now == 0.f) continue;  // nothing but -inf so far
+    o *= was / now;
+    const float w = p / now;
+    for (int t0 = 0; t0 < 64; t0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        x[u] = Elem<T>::to_f32(vbase[(int64_t)__builtin_amdgcn_readlane(page, t0 + u) * page_elems + __builtin_amdgcn_readlane(at, t0 + u) + e]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (__builtin_amdgcn_readlane((int)vis, t0 + u)) o = fmaf(readlane_f32(w, t0 + u), x[u], o);
+    }
+    if (!__any(asked & (o == o))) break;
+  }
+  return l == 0.f ? __builtin_nanf("") : o;
+}
+
+// WHOLE: dh == DHT, no lane is ever outside the head.  SPLIT: parts for the join; a kernel of its own, because what only a whole head needs (pd_exact, the weights)
+// costs the walk scalar registers: 16 sequences, window 1500 (fp32, heads of 96): 65.9 -> 65.1 us
+template <typename T, int DHT, int NW, bool WHOLE, bool NT, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(PagedDecodeArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int TK = pc_tile<T>(), ST = TK / 16;  // 16-key score tiles of a step
@@ -149,15 +207,15 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
   constexpr int VW = DPL * (int)sizeof(T) / 4;    // 32-bit words per lane of a V row
   extern __shared__ float sm[];  // [NW][ng][DHT] outputs, [NW][16][2] (m, l), [16][2] (m, 1 / l), [ng][score_lds] scores
 
-  const int split = blockIdx.x, b = blockIdx.z;
+  const int split = SPLIT ? (int)blockIdx.x : 0, b = blockIdx.z;
   const int kvh = (int)blockIdx.y / a.GT, gt = (int)blockIdx.y - kvh * a.GT;
   const int h0 = kvh * a.G + gt * 16, ng = min(16, a.G - gt * 16);
   const Span<TK> sp = span_of_row<TK>(a, b);
-  const int chunk = split_tiles(sp.tt, a.nsplit), t0 = split * chunk, t1 = min(t0 + chunk, sp.tt);
+  const int chunk = split_tiles(sp.tt, SPLIT ? a.nsplit : 1), t0 = split * chunk, t1 = min(t0 + chunk, sp.tt);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform, and with it everything about a step but the lanes' own places
   const int H = a.Hkv * a.G, ps = 1 << a.psl, dh = WHOLE ? DHT : a.dh;
-  if (split > 0 && t0 >= sp.tt) return;  // nothing of this sequence is left for this split, and the join does not read it
+  if (SPLIT && split > 0 && t0 >= sp.tt) return;  // nothing of this sequence is left for this split, and the join does not read it
 
   float* sm_ml = sm + NW * ng * DHT;
   float* sm_stat = sm_ml + NW * 32;
@@ -284,7 +342,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
         }
     }
     if (a.mass != nullptr && c < ng) {
-      float* sc = a.score_lds ? sm_score + c * a.score_lds + t * TK + 4 * g : a.scores + ((int64_t)b * H + h0 + c) * a.score_ld + (int64_t)t * TK + 4 * g;
+      float* sc = !SPLIT && a.score_lds ? sm_score + c * a.score_lds + t * TK + 4 * g : a.scores + ((int64_t)b * H + h0 + c) * a.score_ld + (int64_t)t * TK + 4 * g;
 #pragma unroll
       for (int st = 0; st < ST; ++st) *reinterpret_cast<pc_f32x4*>(sc + 16 * st) = s[st];
     }
@@ -363,22 +421,31 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 3 : 1) void paged_decode_kernel(
     sm_stat[tid * 2] = ref;
     sm_stat[tid * 2 + 1] = __float_as_uint(L) == 0x80000000u ? 0.f : 1.0f / L;
     if (a.part_ml != nullptr) {
-      float* ml = a.part_ml + (((int64_t)b * H + h0 + tid) * a.nsplit + split) * 2;
+      float* ml = a.part_ml + (((int64_t)b * H + h0 + tid) * (SPLIT ? a.nsplit : 1) + split) * 2;
       ml[0] = M;
       ml[1] = L;
     }
   }
   __syncthreads();
   for (int idx = tid; idx < ng * DHT; idx += NW * 64) {
-    const int hh = idx / DHT, e = idx - hh * DHT;
-    if (!WHOLE && e >= dh) continue;
+    const int hh = idx / DHT, e = idx - hh * DHT;  // (a wave's lanes are in one head: 64 divides DHT)
+    const bool in = WHOLE || e < dh;
     float O = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) O += sm[(i * ng + hh) * DHT + e] * sm_ml[(i * 16 + hh) * 2];
-    if (a.nsplit == 1) store_elem<T>((T*)a.out + ((int64_t)b * H + h0 + hh) * dh + e, O * sm_stat[hh * 2 + 1]);
-    else a.part_o[(((int64_t)b * H + h0 + hh) * a.nsplit + split) * dh + e] = O;
+    if constexpr (!SPLIT) {
+      float x = O * sm_stat[hh * 2 + 1];
+      const bool odd = in & !(fabsf(x) < INFINITY);
+      if (__builtin_expect(__any(odd), 0)) {
+        const float again = pd_exact<T, TK>(a, sp, b, h0 + hh, e, odd);
+        x = odd ? again : x;
+      }
+      if (in) store_elem<T>((T*)a.out + ((int64_t)b * H + h0 + hh) * dh + e, x);
+    } else if (in) {
+      a.part_o[(((int64_t)b * H + h0 + hh) * a.nsplit + split) * dh + e] = O;
+    }
   }
-  if (a.score_lds == 0) return;
+  if (SPLIT || a.score_lds == 0) return;
   for (int idx = tid; idx < sp.tt * TK; idx += NW * 64) {  // the weights of this workgroup's keys and heads
     const int j = sp.key0(idx / TK) + idx % TK;
     if (!sp.sees(j)) continue;
@@ -428,11 +495,16 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(PagedDecodeArgs 
       for (int s = r0; s < used; s += rows) O += *reinterpret_cast<const pc_f32x4*>(a.part_o + (hb * a.nsplit + s) * dh + e) * sh_a[s];
     *reinterpret_cast<pc_f32x4*>(sh_o + tid * 4) = O;
     __syncthreads();
-    for (int i = tid; i < dh; i += 256) {
-      float sum = 0.f;
-      for (int r = 0; r < rows; ++r) sum += sh_o[r * vpr * 4 + i];
-      store_elem<T>((T*)a.out + hb * dh + i, sum * inv);
+    if (w * 64 >= dh) return;
+    float x = 0.f;
+    for (int r = 0; r < rows; ++r) x += sh_o[r * vpr * 4 + min(tid, dh - 1)];
+    x *= inv;
+    const bool odd = (tid < dh) & !(fabsf(x) < INFINITY);
+    if (__builtin_expect(__any(odd), 0)) {
+      const float again = pd_exact<T, TK>(a, sp, b, kvh * a.G + blockIdx.x, tid, odd);
+      x = odd ? again : x;
     }
+    if (tid < dh) store_elem<T>((T*)a.out + hb * dh + tid, x);
     return;
   }
   const int part = (int)blockIdx.x - a.join_heads;
@@ -496,20 +568,21 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
   return p;
 }
 
-template <typename T, int DHT, int NW>
+template <typename T, int DHT, int NW, bool SPLIT>
 static void pd_launch_nw(hipStream_t st, const PagedDecodePlan& p, const PagedDecodeArgs& a, int B) {
   const int ng = std::min(16, a.G);
   const size_t lds = ((size_t)NW * ng * DHT + NW * 32 + 32 + (size_t)ng * p.score_lds) * sizeof(float);
   const dim3 grid(p.nsplit, a.Hkv * a.GT, B), block(NW * 64);
-  if (a.dh != DHT) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, false, false>), grid, block, lds, st, a);
-  else if (p.stream) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, false>), grid, block, lds, st, a);
+  if (a.dh != DHT) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, false, false, SPLIT>), grid, block, lds, st, a);
+  else if (p.stream) hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, true, SPLIT>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((paged_decode_kernel<T, DHT, NW, true, false, SPLIT>), grid, block, lds, st, a);
 }
 
 template <typename T, int DHT>
 static int pd_launch(hipStream_t st, const PagedDecodePlan& p, PagedDecodeArgs& a, int B) {
-  if (p.nw == 8) pd_launch_nw<T, DHT, 8>(st, p, a, B);
-  else pd_launch_nw<T, DHT, 4>(st, p, a, B);
+  if (p.nsplit > 1) pd_launch_nw<T, DHT, 4, true>(st, p, a, B);
+  else if (p.nw == 8) pd_launch_nw<T, DHT, 8, false>(st, p, a, B);
+  else pd_launch_nw<T, DHT, 4, false>(st, p, a, B);
   a.join_heads = p.nsplit > 1 ? a.G : 0;
   const int parts = a.join_heads + (p.score_floats ? (p.tiles * pc_tile<T>() + PD_JOIN_KEYS - 1) / PD_JOIN_KEYS : 0);
   if (parts > 0) hipLaunchKernelGGL((paged_decode_join_kernel<T>), dim3(parts, a.Hkv, B), dim3(256), 0, st, a);
