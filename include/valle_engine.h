@@ -396,7 +396,8 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  *   keys with the largest mass (of equal ones the earlier; NaN counts as the largest), per key-value head, `budget` in all; text_len beyond the
  *   budget takes all of it, and what it leaves bounds `recent`.  The keys that stay move up in order, in place, with their mass.
  *   kept int32 [B][nhead_kv][budget]: their old positions, ascending (-1 past the end); new_lengths int32 [B] = min(lengths, budget).
- *   A page stands in the tables once here. */
+ *   A page stands in the tables once here.  The pools, mass, kept and new_lengths overlap neither each other nor the tables and lengths (VLE_EINVAL):
+ *   in particular new_lengths is not lengths_dev, which is read to the end of the call. */
 int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                             int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
                             const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,

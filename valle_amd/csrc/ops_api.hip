@@ -312,6 +312,32 @@ static int op_refuse(const char* op, const char* why) {
   return op_fail(msg);
 }
 
+// Memory that a call takes: `bytes` from p on (null or none: nothing).
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+// Whether something that a call writes overlaps something else that it takes.
+template <size_t NW, size_t NR>
+static bool overlapping(const Range (&written)[NW], const Range (&read)[NR]) {
+  auto meet = [](const Range& a, const Range& b) {
+    if (!a.p || !b.p || a.bytes <= 0 || b.bytes <= 0) return false;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x <= y ? y - x < (uintptr_t)a.bytes : x - y < (uintptr_t)b.bytes;
+  };
+  for (size_t i = 0; i < NW; ++i) {
+    for (size_t j = i + 1; j < NW; ++j)
+      if (meet(written[i], written[j])) return true;
+    for (size_t j = 0; j < NR; ++j)
+      if (meet(written[i], read[j])) return true;
+  }
+  return false;
+}
+static const char* OVERLAP = "what is written must not overlap another operand";
+static int64_t pool_bytes(int dtype, int32_t n_pages, int32_t nhead_kv, int32_t page_size, int32_t dh) {  // a page has fewer than 2^30 elements (cache_fault): fits
+  return (int64_t)nhead_kv * page_size * dh * (dtype == DT_F32 ? 4 : 2) * n_pages;
+}
+
 extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                        int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
                                        const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,
@@ -410,8 +436,11 @@ extern "C" int vle_op_kv_evict(void* stream, int dtype, void* k_pages, void* v_p
   if (recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget) return op_refuse(op, "sinks and recent keys must fit the budget");
   if (B == 0) return VLE_OK;
   if (!k_pages || !v_pages || !mass || !page_table_dev || !lengths_dev || !kept || !new_lengths) return op_refuse(op, "null operand");
-  if (k_pages == v_pages) return op_refuse(op, "keys and values need pages of their own");
   if (!aligned16(k_pages) || !aligned16(v_pages)) return op_refuse(op, "pages must start on 16 bytes");
+  const int64_t pool = pool_bytes(dtype, n_pages, nhead_kv, page_size, dh), index = (int64_t)B * 4;
+  const Range written[] = {{k_pages, pool}, {v_pages, pool}, {mass, (int64_t)n_pages * nhead_kv * page_size * 4}, {kept, index * nhead_kv * budget}, {new_lengths, index}};
+  const Range read[] = {{page_table_dev, index * table_width}, {lengths_dev, index}, {text_len_dev, index}};
+  if (overlapping(written, read)) return op_refuse(op, OVERLAP);  // new_lengths over lengths too: the move goes by the lengths that the selection saw
   EvictArgs a;
   a.k_pages = k_pages; a.v_pages = v_pages; a.mass = mass; a.table = page_table_dev; a.lengths = lengths_dev; a.text_len = text_len_dev;
   a.kept = kept; a.new_lengths = new_lengths; a.Hkv = nhead_kv; a.n_pages = n_pages; a.W = table_width; a.psl = log2_of(page_size);
