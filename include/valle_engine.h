@@ -382,6 +382,9 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  * what index arrays hold is bounded inside the kernels: offsets and lengths are clamped to the rows / the table, and a page id outside
  * [0, n_pages) is never followed -- its keys are absent.  The HIP device current at the call must be the stream's.
  * Nothing is allocated and nothing waits: every call can be captured into a graph.
+ * What a call writes (out, workspace, pools, mass, kept, new_lengths) must not overlap any other operand, from the first to the last element that its strides
+ * reach; such a call is refused.  Operands that are only read may share memory, and k / v of vle_op_paged_kv_write may be views of the pools, as long as no slot is
+ * both read and written.
  *
  * vle_op_window_attention: packed sequences, rows seq_off[b] .. seq_off[b + 1] - 1 of q / k / v [rows][heads][dh]; out T [rows][nhead][dh].
  *   Rows that no sequence holds are left as they were, or set to 0 where zero_rest != 0.  text_len may be NULL (0).
@@ -396,8 +399,7 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  *   keys with the largest mass (of equal ones the earlier; NaN counts as the largest), per key-value head, `budget` in all; text_len beyond the
  *   budget takes all of it, and what it leaves bounds `recent`.  The keys that stay move up in order, in place, with their mass.
  *   kept int32 [B][nhead_kv][budget]: their old positions, ascending (-1 past the end); new_lengths int32 [B] = min(lengths, budget).
- *   A page stands in the tables once here.  The pools, mass, kept and new_lengths overlap neither each other nor the tables and lengths (VLE_EINVAL):
- *   in particular new_lengths is not lengths_dev, which is read to the end of the call. */
+ *   A page stands in the tables once here.  new_lengths is not lengths_dev, which is read to the end of the call. */
 int vle_op_window_attention(void* stream, int dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                             int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, const int32_t* seq_off_dev,
                             const int32_t* text_len_dev, int64_t rows, int32_t B, int32_t nhead, int32_t nhead_kv, int32_t dh,

@@ -333,6 +333,11 @@ static bool overlapping(const Range (&written)[NW], const Range (&read)[NR]) {
   }
   return false;
 }
+// of a (rows, heads, dh) operand with strides in elements
+static int64_t span_bytes(int dtype, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dh) {
+  const __int128 n = ((__int128)(rows - 1) * row + (__int128)(heads - 1) * head + dh) * (dtype == DT_F32 ? 4 : 2);
+  return n > INT64_MAX ? INT64_MAX : (int64_t)n;
+}
 static const char* OVERLAP = "what is written must not overlap another operand";
 static int64_t pool_bytes(int dtype, int32_t n_pages, int32_t nhead_kv, int32_t page_size, int32_t dh) {  // a page has fewer than 2^30 elements (cache_fault): fits
   return (int64_t)nhead_kv * page_size * dh * (dtype == DT_F32 ? 4 : 2) * n_pages;
@@ -352,6 +357,10 @@ extern "C" int vle_op_window_attention(void* stream, int dtype, const void* q, i
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !vec_strides(dtype, q_row, q_head) ||
       !vec_strides(dtype, k_row, k_head) || !vec_strides(dtype, v_row, v_head))
     return op_refuse(op, "rows and heads must start on 16 bytes, rows less than 2^24 elements apart");
+  const Range written[] = {{out, span_bytes(dtype, rows, (int64_t)nhead * dh, nhead, dh, dh)}};
+  const Range read[] = {{q, span_bytes(dtype, rows, q_row, nhead, q_head, dh)}, {k, span_bytes(dtype, rows, k_row, nhead_kv, k_head, dh)},
+                        {v, span_bytes(dtype, rows, v_row, nhead_kv, v_head, dh)}, {seq_off_dev, ((int64_t)B + 1) * 4}, {text_len_dev, (int64_t)B * 4}};
+  if (overlapping(written, read)) return op_refuse(op, OVERLAP);
   WindowAttnArgs a;
   a.q = q; a.k = k; a.v = v; a.out = out;
   a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
@@ -377,6 +386,13 @@ extern "C" int vle_op_paged_kv_write(void* stream, int dtype, const void* k, int
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || !vec_strides(dtype, k_row, k_head) ||
       !vec_strides(dtype, v_row, v_head))
     return op_refuse(op, "rows and heads must start on 16 bytes, rows less than 2^24 elements apart");
+  // (k and v are not among these: rows may come out of other pages of the same pools)
+  const int64_t pool = pool_bytes(dtype, n_pages, nhead_kv, page_size, dh), index = (int64_t)B * 4, mass_bytes = (int64_t)n_pages * nhead_kv * page_size * 4;
+  const Range written[] = {{k_pages, pool}, {v_pages, pool}, {mass, mass_bytes}};
+  const Range read[] = {{page_table_dev, index * table_width}, {start_dev, index}, {seq_off_dev, index + 4}};
+  const Range weights[] = {{mass, mass_bytes}};
+  const Range rows_read[] = {{k, span_bytes(dtype, rows, k_row, nhead_kv, k_head, dh)}, {v, span_bytes(dtype, rows, v_row, nhead_kv, v_head, dh)}};
+  if (overlapping(written, read) || overlapping(weights, rows_read)) return op_refuse(op, OVERLAP);
   PagedWriteArgs a;
   a.k = k; a.v = v; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
   a.k_pages = k_pages; a.v_pages = v_pages; a.mass = mass; a.table = page_table_dev; a.start = start_dev; a.seq_off = seq_off_dev;
@@ -413,6 +429,10 @@ extern "C" int vle_op_paged_decode_attention(void* stream, int dtype, const void
   const PagedDecodePlan p = paged_decode_plan(dtype, B, nhead_kv, nhead / nhead_kv, dh, table_width, page_size, window, sinks, text_len_dev != nullptr, mass != nullptr);
   const int64_t need = (int64_t)(p.ml_floats + p.o_floats + p.score_floats) * (int64_t)sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need)) return op_refuse(op, "workspace too small (vle_op_paged_decode_workspace_bytes)");
+  const int64_t pool = pool_bytes(dtype, n_pages, nhead_kv, page_size, dh), index = (int64_t)B * 4;
+  const Range written[] = {{out, span_bytes(dtype, B, (int64_t)nhead * dh, nhead, dh, dh)}, {mass, (int64_t)n_pages * nhead_kv * page_size * 4}, {workspace, need}};
+  const Range read[] = {{q, span_bytes(dtype, B, q_row, nhead, q_head, dh)}, {k_pages, pool}, {v_pages, pool}, {page_table_dev, index * table_width}, {lengths_dev, index}, {text_len_dev, index}};
+  if (overlapping(written, read)) return op_refuse(op, OVERLAP);
   PagedDecodeArgs a;
   a.q = q; a.q_b = q_row; a.q_h = q_head; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.mass = mass;
   a.table = page_table_dev; a.lengths = lengths_dev; a.text_len = text_len_dev;

@@ -474,7 +474,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     q (rows, H, dh), k / v (rows, Hkv, dh), H a multiple of Hkv, fp32 | bf16, strided views welcome (e.g. the slices of one packed qkv);
     seq_off int32 (B + 1,), text_len int32 (B,) or None.  Row i sees the keys j < text_len[b] (a prefix-LM's text), and of the keys up to i the
     last `window` (0: all) and the first `sinks`.  scale defaults to 1 / sqrt(dh).  Returns out (rows, H, dh); rows that no sequence
-    holds are 0, or left as they were in a given `out` (which must not overlap the operands).  A key that a row does not see cannot
+    holds are 0, or left as they were in a given `out` (refused where its memory overlaps an operand's, from the first to the last element).  A key that a row does not see cannot
     reach it, whatever it holds.  No synchronization; forward only."""
     who = "window_attention"
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
@@ -506,7 +506,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     k / v (rows, Hkv, dh), strided views welcome; k_pages / v_pages (n_pages, Hkv, page_size, dh) of the same type; page_table int32 (B, W):
     key j of sequence b lives in page page_table[b][j // page_size] (a power of two, >= 8), slot j % page_size.  Row r of sequence b (rows
     seq_off[b] .. seq_off[b + 1] - 1; None: one row each) becomes key start[b] + r - seq_off[b]; mass (n_pages, Hkv, page_size) fp32 becomes 0 there.
-    Rows of no sequence, positions past the table and page ids outside the pool are dropped; two rows must not go to one slot."""
+    Rows of no sequence, positions past the table and page ids outside the pool are dropped; two rows must not go to one slot.  k and v may be views of
+    the pools (a page copied to another), as long as no slot is both read and written."""
     who = "paged_kv_write"
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
     rows = k.shape[0] if k.dim() == 3 else 0
@@ -543,7 +544,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     q (B, H, dh), a strided view welcome, of the pages' type; lengths int32 (B,): keys of each sequence, its newest (the query's own) included;
     window / sinks / text_len as in window_attention, for row lengths[b] - 1.  Returns out (B, H, dh): 0 where no key is visible (a length of 0).
     mass (n_pages, Hkv, page_size) fp32: every visible key's attention weight, summed over the query heads that share it, is added in place --
-    what kv_evict goes by.  Sequences may share pages (their weights are then added in no fixed order).  The split follows the width of
+    what kv_evict goes by.  Sequences may share pages (their weights are then added in no fixed order).  `out` and mass must not overlap another operand (refused).  The split follows the width of
     page_table: hand a table as wide as the longest sequence needs."""
     who = "paged_decode_attention"
     n_pages, Hkv, ps, dh, B, W = _pages(who, k_pages, v_pages, page_table, mass)
