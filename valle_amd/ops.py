@@ -11,6 +11,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -377,7 +378,7 @@ def linear_fp8(a8: torch.Tensor, a_scale: torch.Tensor, w8: torch.Tensor, w_scal
 
 # ---- attention with a window, and the paged key-value cache (vle_op_window_attention, vle_op_paged_*, vle_op_kv_evict) ------------------
 # Row i of a sequence sees key j iff  j < text_len  or  (j <= i and (window == 0 or i - j < window or j < sinks)).
-# Forward only.  What an index tensor holds is not read on the host (no synchronization, every call can be captured into a graph): the kernels
+# Forward only: operands, masses and outputs that ask for a gradient or carry a tangent are refused.  What an index tensor holds is not read on the host (no synchronization, every call can be captured into a graph): the kernels
 # clamp offsets and lengths and never follow a page id outside the pool.
 def _refuse(who: str, what: str):
     raise ValueError(f"{who}: {what}")
@@ -390,8 +391,8 @@ def _count(who: str, name: str, v: int) -> int:
     return v
 
 
-def _operands(who: str, first: torch.Tensor, *others: torch.Tensor) -> int:
-    """One device, one type, no gradient asked for; -> the type's code."""
+def _operands(who: str, first: torch.Tensor, *others: torch.Tensor, written: tuple = ()) -> int:
+    """One device, one type, no derivative asked for (of `written`, tensors or None, neither); -> the type's code."""
     what, where, grad = first.dtype, first.get_device(), first.requires_grad
     for t in others:
         if t.dtype is not what:
@@ -399,8 +400,12 @@ def _operands(who: str, first: torch.Tensor, *others: torch.Tensor) -> int:
         if t.get_device() != where:
             _refuse(who, "all tensors must be on one device")
         grad = grad or t.requires_grad
+    for t in written:
+        grad = grad or (t is not None and t.requires_grad)
     if grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who} has no backward pass: detach its operands or call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (first, *others, *written)):
+        raise RuntimeError(f"{who} has no forward-mode derivative: its operands' tangents would be lost")
     return _lib.DTYPE_BF16 if what is torch.bfloat16 else _dt(first)
 
 
@@ -486,7 +491,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     if seq_off.dim() != 1 or seq_off.shape[0] < 1:
         _refuse(who, "seq_off must be (B + 1,)")
     B = seq_off.shape[0] - 1
-    dt = _operands(who, q, k, v)
+    dt = _operands(who, q, k, v, written=(out,))
     seq_off = _index(who, "seq_off", seq_off, B + 1, q)
     if text_len is not None:
         text_len = _index(who, "text_len", text_len, B, q)
@@ -517,7 +522,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
         _refuse(who, "keys and values need pages of their own")
     if seq_off is None and rows != B:
         _refuse(who, "without seq_off there is one row per sequence")
-    dt = _operands(who, k, v, k_pages, v_pages)
+    dt = _operands(who, k, v, k_pages, v_pages, written=(mass,))
     start = _index(who, "start", start, B, k)
     if seq_off is not None:
         seq_off = _index(who, "seq_off", seq_off, B + 1, k)
@@ -551,7 +556,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     H = q.shape[1] if q.dim() == 3 else 0
     if q.shape != (B, H, dh) or Hkv < 1 or H < 1 or H % Hkv:
         _refuse(who, "q must be (B, H, dh): the table's sequences, the pages' head size, a multiple of their heads")
-    dt = _operands(who, q, k_pages, v_pages)
+    dt = _operands(who, q, k_pages, v_pages, written=(mass, out))
     lengths = _index(who, "lengths", lengths, B, q)
     if text_len is not None:
         text_len = _index(who, "text_len", text_len, B, q)
@@ -585,7 +590,7 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
         _refuse(who, "keys and values need pages of their own")
     if _count(who, "budget", budget) < 1:
         _refuse(who, "budget must be 1 at least")
-    dt = _operands(who, k_pages, v_pages)
+    dt = _operands(who, k_pages, v_pages, written=(mass,))
     lengths = _index(who, "lengths", lengths, B, k_pages)
     if text_len is not None:
         text_len = _index(who, "text_len", text_len, B, k_pages)
