@@ -1,5 +1,5 @@
-"""CPU: what the cache operators owe autograd, though they have no backward pass: gradients and tangents that would be lost are refused.  (Refusals come before
-anything else; for the rest the C entries are left out.)"""
+"""CPU: what the cache operators owe autograd, though they have no backward pass: gradients and tangents that would be lost are refused, tensors written in place
+count as written.  (Refusals come before anything else; for the rest the C entries are left out.)"""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -52,6 +52,28 @@ def test_tensors_with_a_tangent_are_refused(op, name, monkeypatch):
         monkeypatch.setattr(ops, "_call", lambda *a: None)
         t[name] = forward_ad.unpack_dual(t[name]).primal
         call()
+
+
+@pytest.mark.parametrize("op,written", [("window", {"out"}), ("write", {"k_pages", "v_pages", "mass"}), ("decode", {"mass", "out"}), ("evict", {"k_pages", "v_pages", "mass"})])
+def test_tensors_written_in_place_count_as_written(op, written, monkeypatch):
+    """Saved for a backward pass and overwritten by one of these operators, a tensor has to be found out."""
+    monkeypatch.setattr(ops, "_call", lambda *a: None)
+    t = operands()
+    was = {n: x._version for n, x in t.items()}
+    call, names = calls(t)[op]
+    call()
+    for n in names:
+        assert (t[n]._version > was[n]) == (n in written), n
+    x = torch.ones(3, requires_grad=True)
+    for n in written:
+        y = (x.sum() * t[n]).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        t = operands()
+        calls(t)[op][0]()
+    calls(t)[op][0]()  # tensors of inference mode, which count nothing
 
 
 def test_optional_tensors_may_be_missing(monkeypatch):

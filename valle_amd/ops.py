@@ -472,6 +472,11 @@ def _call(t: torch.Tensor, entry: str, *args) -> None:
         _lib.check(rc)
 
 
+def _wrote(*tensors: Optional[torch.Tensor]) -> None:
+    """Memory that a C entry wrote counts as written: a backward pass that saved one of these tensors finds out."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: torch.Tensor, window: int = 0, sinks: int = 0,
                      text_len: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of packed sequences with a sliding window, first tokens that stay visible and grouped heads.
@@ -501,6 +506,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     _call(q, "vle_op_window_attention", dt, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, o.data_ptr(), seq_off.data_ptr(),
           None if text_len is None else text_len.data_ptr(), rows, B, H, Hkv,
           dh, _count(who, "window", window), _count(who, "sinks", sinks), dh ** -0.5 if scale is None else scale, out is None)
+    if out is not None:
+        _wrote(out)
     return o
 
 
@@ -531,6 +538,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     _call(k, "vle_op_paged_kv_write", dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, k_pages.data_ptr(), v_pages.data_ptr(),
           None if mass is None else mass.data_ptr(), page_table.data_ptr(), start.data_ptr(), None if seq_off is None else seq_off.data_ptr(), rows,
           B, Hkv, dh, n_pages, W, ps)
+    _wrote(k_pages, v_pages, mass)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -570,6 +578,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
           lengths.data_ptr(), None if text_len is None else text_len.data_ptr(), None if mass is None else mass.data_ptr(), ws.data_ptr() if room else None, room, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
           dh ** -0.5 if scale is None else scale)
+    if mass is not None or out is not None:
+        _wrote(mass, out)
     return o
 
 
@@ -599,4 +609,5 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     _call(k_pages, "vle_op_kv_evict", dt, k_pages.data_ptr(), v_pages.data_ptr(), mass.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
           None if text_len is None else text_len.data_ptr(), kept.data_ptr(), left.data_ptr(), B, Hkv, dh, n_pages, W, ps, budget,
           _count(who, "recent", recent), _count(who, "sinks", sinks))
+    _wrote(k_pages, v_pages, mass)
     return kept, left
