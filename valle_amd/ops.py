@@ -401,7 +401,8 @@ def _operands(who: str, first: torch.Tensor, *others: torch.Tensor, written: tup
             _refuse(who, "all tensors must be on one device")
         grad = grad or t.requires_grad
     for t in written:
-        grad = grad or (t is not None and t.requires_grad)
+        if t is not None and t.requires_grad:
+            grad = True
     if grad and torch.is_grad_enabled():
         raise RuntimeError(f"{who} has no backward pass: detach its operands or call it under torch.no_grad()")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (first, *others, *written)):
@@ -472,9 +473,9 @@ def _call(t: torch.Tensor, entry: str, *args) -> None:
         _lib.check(rc)
 
 
-def _wrote(*tensors: Optional[torch.Tensor]) -> None:
+def _wrote(*tensors: torch.Tensor) -> None:
     """Memory that a C entry wrote counts as written: a backward pass that saved one of these tensors finds out."""
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    torch._C._increment_version(tensors)  # torch.autograd.graph.increment_version without its wrapper
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: torch.Tensor, window: int = 0, sinks: int = 0,
@@ -538,7 +539,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     _call(k, "vle_op_paged_kv_write", dt, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, k_pages.data_ptr(), v_pages.data_ptr(),
           None if mass is None else mass.data_ptr(), page_table.data_ptr(), start.data_ptr(), None if seq_off is None else seq_off.data_ptr(), rows,
           B, Hkv, dh, n_pages, W, ps)
-    _wrote(k_pages, v_pages, mass)
+    _wrote(k_pages, v_pages) if mass is None else _wrote(k_pages, v_pages, mass)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -578,8 +579,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     _call(q, "vle_op_paged_decode_attention", dt, q.data_ptr(), qr, qh, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
           lengths.data_ptr(), None if text_len is None else text_len.data_ptr(), None if mass is None else mass.data_ptr(), ws.data_ptr() if room else None, room, o.data_ptr(), B, H, Hkv, dh, n_pages, W, ps, window, sinks,
           dh ** -0.5 if scale is None else scale)
-    if mass is not None or out is not None:
-        _wrote(mass, out)
+    if mass is not None:
+        _wrote(mass)
+    if out is not None:
+        _wrote(out)
     return o
 
 
