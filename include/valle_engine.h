@@ -387,12 +387,13 @@ int vle_op_adaln_fold(void* stream, const float* wb, const float* g, const float
  * both read and written.
  *
  * vle_op_window_attention: packed sequences, rows seq_off[b] .. seq_off[b + 1] - 1 of q / k / v [rows][heads][dh]; out T [rows][nhead][dh].
- *   Rows that no sequence holds are left as they were, or set to 0 where zero_rest != 0.  text_len may be NULL (0).
+ *   Rows that no sequence holds are left as they were, or set to 0 where zero_rest != 0.  text_len may be NULL (0).  bf16: the softmax weights are rounded to bf16
+ *   in numerator and denominator alike (scores, maxima and sums are fp32 in both types).
  * vle_op_paged_kv_write: row r of sequence b (seq_off as above, or NULL: row b alone) becomes key start[b] + r - seq_off[b], in slot
  *   pos % page_size of page page_table[b][pos / page_size] of k_pages / v_pages T [n_pages][nhead_kv][page_size][dh]; its mass (NULL or f32
- *   [n_pages][nhead_kv][page_size]) becomes 0.  Positions past the table are dropped.  page_size: a power of two, >= 8.
+ *   [n_pages][nhead_kv][page_size]) becomes 0, which for the keys of a prompt it stays until a decode step adds to it.  Positions past the table are dropped.  page_size: a power of two, >= 8.
  * vle_op_paged_decode_attention: q T [B][nhead][dh], the newest token of sequence b is key lengths[b] - 1; out T [B][nhead][dh] (0 where no
- *   key is visible).  mass != NULL: += the weight every visible key received, summed over the query heads of its key-value head.
+ *   key is visible); window counts cache slots, after an eviction too.  bf16: weights of 16 bits.  mass != NULL: += the weight every visible key received, summed over the query heads of its key-value head.
  *   Sequences may share pages (their weights are then added in no fixed order).  workspace: vle_op_paged_decode_workspace_bytes(...) bytes
  *   (may be 0) on 16 bytes, not used by another call at the same time.
  * vle_op_kv_evict: sequences of more than `budget` keys keep the first max(text_len, sinks), the last `recent` and, of those between, the

@@ -30,7 +30,8 @@ template <int TK>
 struct Span {
   int n, hd, lo, th, mf, tt;
   __device__ int key0(int t) const { return (t < th ? t : mf + (t - th)) * TK; }
-  // (& and | on purpose: a select per key, no branches)
+  // & and | on purpose, here and where a mask is applied.  Not for speed: with && and || (a branch inside a step that only some waves take) hipcc of ROCm 7.2 left element 0
+  // of a vector of scores unmasked for keys in the gap ahead of the window.  A select for every key is compiled right, behind a wave-uniform branch too.
   __device__ bool sees(int j) const { return (j < n) & ((j < hd) | (j >= lo)); }
   __device__ bool sees_tile(int j0) const { return (j0 + TK <= n) & ((j0 + TK <= hd) | (j0 >= lo)); }
 };
@@ -111,9 +112,9 @@ int launch_paged_write(hipStream_t st, int dtype, const PagedWriteArgs& a) {
 // them into the operands of DPL products, product j giving dims 4-lane-slot * DPL + j.  No LDS, no barrier in the loop; a group of one
 // head leaves 15 columns empty, which the matrix pipe has room for (it needs 1/16 of the time the HBM takes for the same keys).
 //
-// HBM-bound.  Measured: 3 sequences of 40k - 60k keys, 32 heads on 8 of 128, bf16 (684 MB): 110 us = 6.2 TB/s, and 4.7 the join; 16 sequences, window 1500
-// of 9k - 30k keys, 16 heads of 96, fp32 (312 MB): 60 us = 5.2 TB/s, and 4.7; 64 sequences of 330 - 1100 keys, 16 heads of 64, with mass (216 MB): 50 us = 4.3
-// TB/s, bound by the longest sequences, whose workgroups run on alone; one sequence of 1025 keys: 10.2 us, the steps' latency one after another.
+// HBM-bound.  Measured: 3 sequences of 40k - 60k keys, 32 heads on 8 of 128, bf16 (684 MB): 111 us = 6.2 TB/s, and 4.9 the join; 16 sequences, window 1500
+// of 9k - 30k keys, 16 heads of 96, fp32 (312 MB): 60 us = 5.2 TB/s, and 4.9; 64 sequences of 330 - 1100 keys, 16 heads of 64, with mass (216 MB): 50 us = 4.3
+// TB/s, bound by the longest sequences, whose workgroups run on alone; one sequence of 1025 keys: 9.8 us, the steps' latency one after another.
 // A second tile of registers on its way is slower, also where workgroups are few (138 -> 141 us and 73 -> 87 for the first two, at the time; 10.2 -> 10.6
 // for the last).
 
@@ -546,17 +547,19 @@ PagedDecodePlan paged_decode_plan(int dtype, int B, int Hkv, int G, int dh, int 
   // caches with 8 heads take 113 us, 43 (one third more than fit) 128, 64 (two rounds) 116, 128 (shorter parts, a longer join) 121.
   const int64_t slots = 256 * (dh <= 64 ? 5 : 3);
   p.nsplit = 1;
-  // 8 waves where groups are few (their outputs fit 32 KB of LDS for up to 8 heads): one sequence of 600 keys, 16 heads of 64, 6.9 us, with 4 waves 9.6;
-  // 16 sequences of 2000: 27 / 37; 24 of 1000: 24 / 23; 64 sequences: no difference
+  // 8 waves where groups are few (their outputs fit 32 KB of LDS for up to 8 heads), 8 / 4 in a graph, 16 heads of 64: one sequence of 600 keys 6.6 / 8.9 us; 16 of 2000
+  // 26.7 / 34.4; 24 of 1000 23.2 / 22.0; 32 of 2000 45.0 / 46.1; 64 sequences: no difference.  fp32: 12.3 / 16.6, 43.9 / 63.2, 42.0 / 39.5, 84.9 / 82.4
   p.nw = groups < 512 && ng <= 8 ? 8 : 4;
-  // One workgroup a head takes 7 us per 1000 keys of 64 (a CU alone pulls about 40 GB/s), the join costs 3 us and a launch on the host: one sequence of
-  // 16 heads of 64 is faster unsplit up to 1040 keys (10.7 / 14.0 us a call), split from 1500 on (13.6 / 13.8; 13.8 / 10.0 in a graph).  A group for
-  // every CU needs no split yet at 2000 keys (16 sequences, 16 heads: 27 / 31 us).
+  // One workgroup a head takes 7 us per 1000 keys of 64 (a CU alone pulls about 40 GB/s), the join costs 3 us and a launch on the host.  16 heads of 64, unsplit / split:
+  // one sequence of 1040 keys 10.0 / 14.4 us a call (9.1 / 8.8 in a graph), of 1300 10.8 / 15.0 (10.5 / 8.9), of 1500 11.6 / 14.8 (11.4 / 9.3), of 2040 14.7 / 14.8 (14.8 / 9.6);
+  // fp32, whose tiles have half the keys, of 600 12.5 / 14.3 (12.3 / 9.3), of 1040 19.2 / 14.8.  A group for every CU needs no split yet at 2000 keys (16
+  // sequences: 27.8 / 32.0 us, fp32 47.5 / 50.3), nor do two (32 of 2000: 47.8 / 52.2) or four (64 of 600: 29.3 / 29.3), for sequences of equal lengths.
   if (groups < 512 && p.tiles > (groups < 256 ? 5 : 16) * p.nw) {
     p.nw = 4;
     p.nsplit = (int)std::min((int64_t)std::min(PD_MAX_SPLIT, (p.tiles + PD_CHUNK - 1) / PD_CHUNK), std::max((int64_t)1, slots / groups));
   }
-  // past the memory-side cache where the keys do not fit: 684 MB 126 -> 115 us; 4 MB that would have stayed there: 10.6 -> 11.4
+  // past the memory-side cache where the keys do not fit: 585 MB 114 -> 99 us, 250 MB 50.7 -> 46.2; 31 MB that would have stayed there 10.8 -> 14.1.  Head sizes 64 and 128
+  // alone have a kernel for it: at 96 it made no difference (fp32, 750 MB 141.8 / 142.4; bf16, 375 MB 73.9 / 71.5)
   p.stream = (int64_t)p.tiles * tk * B * Hkv * dh * (dtype == DT_F32 ? 8 : 4) > (int64_t)128 << 20;
   // weights: by the workgroup that has all of a head's scores, where they fit beside its outputs; else by the join (64 sequences of 330 - 1100 keys,
   // 16 heads: 50 us, by the join 56)
@@ -604,7 +607,7 @@ int launch_paged_decode(hipStream_t st, int dtype, const PagedDecodePlan& p, Pag
 // Which keys stay: the first S and the last R of n, and of the n - S - R between them the M = budget - S - R with the most weight (of equal
 // weights the earlier).  One workgroup per (sequence, head) finds the M-th largest weight by three counting passes over its order-preserving
 // 32-bit key (11 + 11 + 10 bits, 2048 counters in LDS), then numbers the keys that stay in one more pass in the order of their positions.
-// Bound by the passes' latency: 4 sequences of 900 - 1500 keys, 16 heads: 8 us; 32 sequences of 4.5k - 9k keys, 8 heads: 21 us.
+// Bound by the passes' latency: 4 sequences of 900 - 1500 keys, 16 heads: 7.2 us; 32 sequences of 4.5k - 9k keys, 8 heads: 16 - 21 us.
 constexpr int EV_T = 1024, EV_NW = EV_T / 64, EV_BINS = 2048;
 
 __device__ inline uint32_t ev_key(float m) {  // larger weight, larger key; NaN above everything, -0 = +0
@@ -761,8 +764,8 @@ __global__ __launch_bounds__(EV_T) void kv_evict_select_kernel(EvictArgs a) {
 // (or a slice of them) by ONE workgroup: a chunk's targets lie below every later chunk's sources, so the next chunk may be on its way while this
 // one is stored, and only the rows of one chunk can overwrite each other's sources -- a barrier between its loads' return and its stores rules
 // that out.  HBM-bound: two chunks of 32 KB in flight per workgroup.  1024 threads of 2 vectors a chunk: 32 sequences of 4.5k - 9k keys, 8 heads of 128,
-// back to 4096, together with the selection 268 us (1.09 GB, 4.1 TB/s; a plain copy reaches 4.9 here); 256 threads of 8 vectors, whose chunk takes as
-// many bytes but whose lanes walk it alone: 302.
+// back to 4096, 211 us, and the selection 16 (1.09 GB in all: 4.8 TB/s, the rate of a large copy); with 256 threads of 8 vectors, whose chunk takes as
+// many bytes but whose lanes walk it alone, both together, timed by events behind other work, 302 for 268.
 constexpr int MV_T = 1024, MV_U = 2, MV_TAB = 4096;
 
 template <bool CACHED, typename V>  // CACHED: the sequence's pages are in LDS

@@ -267,12 +267,14 @@ struct Stager {
 // ---- bf16 --------------------------------------------------------------------------------------------------------------------------
 // 4 waves, QW query fragments of 16 rows each; 64-key tiles of K and V go global -> LDS by DMA into one of two buffers while the other is
 // multiplied (a third buffer changed nothing); V^T operands come from the row-major tile through the transposing LDS read.  The row sums ride on the
-// matrix pipe (an all-ones row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16 (8 bits: 2^-9 of each weight,
-// which averages out over the keys and stays below the output's own rounding).
+// matrix pipe (an all-ones row block of V^T), so numerator and denominator carry the same rounding of the weights to bf16: 2^-8 of each weight at most, which
+// averages out over the keys.  It moves an output by 0.0003 (long rows) to 0.0006 of its size (a few keys), against the 0.0017 of the output's own rounding to
+// bf16: in all 0.0017 - 0.0018 from the exact result, where weights of 32 bits give 0.0016 - 0.0017.  Weights of 16 bits, as the sum of two bf16 numbers, would take
+// the second product twice, which is half of what the matrix pipe does here.
 //
-// Measured: one sequence of 12289 rows, 16 heads on 4 key-value heads of 128, window 2048: 220 us = 860 TFLOP/s of visible pairs, 71 % of what a large
+// Measured: one sequence of 12289 rows, 16 heads on 4 key-value heads of 128, window 2048: 211 - 216 us = 875 - 898 TFLOP/s of visible pairs, 73 % of what a large
 // library product reaches here (1206).  The matrix pipe is busy 41 % of the cycles, the vector pipe 39 % (exponentials, masks, conversions), LDS 20 %; two
-// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 94 us (238 MB; a copy of it takes 49): vector pipe
+// waves a SIMD overlap them in part only.  32 sequences of 700 - 1100 rows, 16 heads of 64, window 256: 91 - 94 us (238 MB; a copy of it takes 49): vector pipe
 // 51 %, matrix pipe 21 %, the rest waits -- a wave of 16 rows computes 460 keys a row for 340 visible ones, head size 64 has half the product per
 // exponential, and walks of 8 tiles do not hide their start.  Two short sequences: 5.0 us, less than a launch costs the host.
 template <int DHT, int QW>
@@ -700,15 +702,16 @@ int launch_window_attention(hipStream_t st, int dtype, const WindowAttnArgs& a) 
   const bool f32 = dtype == DT_F32;
   // items of a head: the rows' runs, one more for every sequence's ragged last one, one for the rows of no sequence
   auto items = [&](int qb) { return (a.rows + qb - 1) / qb + a.B + 1; };
-  // bf16, head size above 96, two workgroups a CU or more: 128 rows each, so that a fragment read from LDS feeds two products (32 heads of 128, sequences of
-  // 1000 rows: 1 of them 26.5 us with 64 rows / 32 with 128, 2: 42 / 38, 8: 125 / 116; 12289 rows, 16 heads: 705 / 579; all before the items' present order).  Smaller heads lose more by the
-  // registers than they win (16 sequences, 16 heads of 96: 91 / 98; 32 of 900, 16 heads of 64, window 256: 73 / 80, no window 107 / 119).
+  // bf16, head size above 96, two workgroups a CU or more: 128 rows each, so that a fragment read from LDS feeds two products (no window, 32 heads of 128, sequences
+  // of 1000 rows, 64 rows an item / 128: 1 of them (320 items of 128) 20.1 / 27.5 us, 2 (608) 33.1 / 31.2, 4 (1184) 59.5 / 59.2, 8 110 / 103; one of 12289 rows, 16
+  // heads: 714 / 599, window 1024 145 / 123; 8 of 1000, 16 heads of 120: 71.5 / 62.9).  Smaller heads win nothing by it (16 of 1000, 16 heads of 96: 88.2 / 89.1, window 256
+  // 59.8 / 62.0; 32 of 900, 16 heads of 64: 106.9 / 108.9, window 256 72.7 / 75.8).
   const bool wide = !f32 && a.dh > 96 && items(128) * a.H >= 512;
   const int64_t n = items(wide ? 128 : 64) * a.H;
   // fp32, about one workgroup a CU (without a window, where the late rows' work is the longest and goes first, up to one and a half): a second group of waves
-  // halves each one's walk.  One sequence, 16 heads of 96, no window: 1300 rows 103 -> 80 us, 1600 131 -> 97, but 2000 141 -> 167; window 256: 1024 rows
-  // 28 -> 27, but 1300 42 -> 48, where a second workgroup a CU is worth more.  (16-key tiles, which leave room for it, are slower from 300 rows to 16 sequences:
-  // 58 / 61, 302 / 336.)
+  // halves each one's walk.  16 heads of 96, one group / two: no window, one sequence of 1300 rows (368 items) 103.5 / 80.8 us, of 1600 (432) 131.9 / 97.0, but of 2000 (544)
+  // 141.8 / 167.4; window 256, 1024 rows (288) 28.9 / 27.4, but 1152 (320) 33.4 / 35.8 and 1300 41.8 / 47.8, where a second workgroup a CU is worth more.  (16-key tiles, which
+  // leave room for it, are slower from 300 rows to 16 sequences: 58 / 61, 302 / 336.)
   const bool pair = f32 && n <= (a.window > 0 ? 320 : 448);
   if (n > 0xffffff) return -1;  // 2^32 work items
   const dim3 grid((unsigned)n), block(256);

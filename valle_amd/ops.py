@@ -485,8 +485,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off:
     q (rows, H, dh), k / v (rows, Hkv, dh), H a multiple of Hkv, fp32 | bf16, strided views welcome (e.g. the slices of one packed qkv);
     seq_off int32 (B + 1,), text_len int32 (B,) or None.  Row i sees the keys j < text_len[b] (a prefix-LM's text), and of the keys up to i the
     last `window` (0: all) and the first `sinks`.  scale defaults to 1 / sqrt(dh).  Returns out (rows, H, dh); rows that no sequence
-    holds are 0, or left as they were in a given `out` (refused where its memory overlaps an operand's, from the first to the last element).  A key that a row does not see cannot
-    reach it, whatever it holds.  No synchronization; forward only."""
+    holds are 0, or left as they were in a given `out` (refused where its memory overlaps an operand's, from the first to the last element).  A key that a row does not
+    see cannot reach it, whatever it holds.  Scores, maxima and sums are fp32; in bf16 the softmax weights are rounded to bf16 (numerator and denominator alike, 2^-8 of a weight
+    at most: 0.0003 to 0.0006 of an output, whose own rounding is 0.0017), in fp32 nothing is.  The weights that the keys receive are not reported: the mass of a prompt's keys
+    stays what paged_kv_write made it, 0.  No synchronization; forward only."""
     who = "window_attention"
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
         _refuse(who, "q must be (rows, H, dh), k and v (rows, Hkv, dh)")
@@ -518,7 +520,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
 
     k / v (rows, Hkv, dh), strided views welcome; k_pages / v_pages (n_pages, Hkv, page_size, dh) of the same type; page_table int32 (B, W):
     key j of sequence b lives in page page_table[b][j // page_size] (a power of two, >= 8), slot j % page_size.  Row r of sequence b (rows
-    seq_off[b] .. seq_off[b + 1] - 1; None: one row each) becomes key start[b] + r - seq_off[b]; mass (n_pages, Hkv, page_size) fp32 becomes 0 there.
+    seq_off[b] .. seq_off[b + 1] - 1; None: one row each) becomes key start[b] + r - seq_off[b]; mass (n_pages, Hkv, page_size) fp32 becomes 0 there (the keys of a
+    prompt too: only paged_decode_attention adds to it).
     Rows of no sequence, positions past the table and page ids outside the pool are dropped; two rows must not go to one slot.  k and v may be views of
     the pools (a page copied to another), as long as no slot is both read and written."""
     who = "paged_kv_write"
@@ -556,7 +559,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """One new query per sequence against its pages, split over the cache's length and joined.
 
     q (B, H, dh), a strided view welcome, of the pages' type; lengths int32 (B,): keys of each sequence, its newest (the query's own) included;
-    window / sinks / text_len as in window_attention, for row lengths[b] - 1.  Returns out (B, H, dh): 0 where no key is visible (a length of 0).
+    window / sinks / text_len as in window_attention, for row lengths[b] - 1, counted in cache slots: after kv_evict the keys that moved up count by their new places, so that
+    a window reaches further back in time.  Scores and sums are fp32, in bf16 the weights keep 16 bits.  A value that is infinite or not a number reaches its own element alone.  Returns out (B, H, dh): 0 where no key is visible (a length of 0).
     mass (n_pages, Hkv, page_size) fp32: every visible key's attention weight, summed over the query heads that share it, is added in place --
     what kv_evict goes by.  Sequences may share pages (their weights are then added in no fixed order).  `out` and mass must not overlap another operand (refused).  The split follows the width of
     page_table: hand a table as wide as the longest sequence needs."""
@@ -593,7 +597,8 @@ def kv_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass: torch.Tensor, p
     Of such a sequence the first max(text_len[b], sinks) keys stay, the last `recent`, and of those between the ones with the largest mass (of
     equal ones the earlier; NaN counts as the largest), `budget` in all, for every key-value head by itself; a text longer than the budget takes all of
     it, and what it leaves bounds `recent`.  They move up in the order they had, with their mass.  Returns (kept int32 (B, Hkv, budget): the old
-    positions, ascending, -1 past the end; lengths int32 (B,) = min(lengths, budget)): the pages behind the new lengths are free.
+    positions, ascending, -1 past the end; lengths int32 (B,) = min(lengths, budget)): the pages behind the new lengths are free.  Keys that no step has weighed yet have mass 0:
+    evicted right after a prompt, the keys between text and recent ones are all equal and the earliest stay.  Masses of the caller's own making may be written there before.
     A page must stand in the tables once, at one place of one sequence."""
     who = "kv_evict"
     if mass is None:
