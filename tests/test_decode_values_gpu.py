@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.test_cache_ops_gpu import DEV, F64, Pool, attend, gen, half_step, i32, near, rnd
+from tests.test_cache_ops_gpu import DEV, F64, Pool, attend, gen, half_step, i32, near, rnd, sees
 from tests.test_window_scores_gpu import LOG2E, scored
 from valle_amd import ops
 
@@ -90,3 +90,51 @@ def test_paged_decode_attention_equal_scores_share_equally(dtype):
             v = pool.v[page, 0, slot].to(F64)
             want = v.mean(0)
             near(got[0], want.expand(2, 64), 2 * (n + 2) * 2.0 ** -24 * v.abs().mean(0) + half_step(dtype) * want.abs(), f"score {score}")
+
+
+@TYPES
+@pytest.mark.parametrize("lens,text,H,Hkv,dh,ps,window,sinks,width", [
+    ([300, 33, 5], [20, 0, 5], 4, 2, 64, 16, 40, 2, None),       # a gap between the head and the window, where everything is NaN
+    ([700, 150], [0, 60], 3, 1, 96, 64, 100, 4, None),
+    ([1500, 900], [0, 17], 4, 2, 64, 8, 700, 3, None),           # split and joined
+    ([900, 64], [70, 0], 40, 2, 40, 16, 333, 0, 300),            # 20 heads a group, a table wider than the sequences
+    ([260], [259], 2, 2, 120, 32, 1, 0, None)])
+def test_paged_decode_attention_extreme_values_behind_a_mask(dtype, lens, text, H, Hkv, dh, ps, window, sinks, width):
+    """Values near the largest number where the newest token looks, infinities and NaN wherever it does not, pages that are not there, queries out of a packed row; then
+    one visible infinity."""
+    g = gen(sum(lens) + window)
+    pool = Pool(g, lens, Hkv, dh, ps, dtype, width=width)
+    pool.table[0, 1] = -3  # keys ps .. 2 ps - 1 of the first sequence
+    n_pages = pool.k.shape[0]
+    packed = rnd(g, len(lens), 3 * H * dh, dtype=dtype, gain=0.3)
+    q = packed[:, H * dh:2 * H * dh].view(-1, H, dh)
+    seen = []
+    for b, n in enumerate(lens):
+        page, slot = pool.at(b)
+        m = sees(n, n - 1, min(text[b], n), window, sinks) & (page >= 0) & (page < n_pages)
+        big = rnd(g, n, Hkv, dh).clamp(-1, 1).mul(3e38).to(dtype)
+        gone, there = ~m & (page >= 0), page >= 0
+        pool.v[page[there], :, slot[there]] = big[there]
+        pool.v[page[gone], :, slot[gone]] = float("nan")
+        pool.v[page[gone], 0, slot[gone]] = float("inf")
+        pool.k[page[gone], :, slot[gone]] = float("nan")
+        seen.append((page, slot, m))
+
+    def check(what):
+        got = ops.paged_decode_attention(packed.to(DEV)[:, H * dh:2 * H * dh].view(-1, H, dh), pool.k.to(DEV), pool.v.to(DEV), pool.table.to(DEV), i32(lens), window=window, sinks=sinks,
+                                         text_len=i32(text)).cpu().to(F64)
+        for b, (page, slot, m) in enumerate(seen):
+            for h in range(H):
+                kh, vh = (x[page.clamp(0), h // (H // Hkv), slot] for x in (pool.k, pool.v))
+                _, _, p, delta = attend(q[b, h], kh, vh.nan_to_num(0.0, 0.0, 0.0), m, 1 / math.sqrt(dh))
+                want, size = (p[:, None] * vh[m].to(F64)).sum(0), (p[:, None] * vh[m].to(F64).abs()).sum(0)
+                fine = want.isfinite()
+                assert torch.equal(got[b, h][~fine], want[~fine]), (what, b, h)
+                rel = 2 * (delta + len(p) * 2.0 ** -24) + (2.0 ** -15 if dtype == torch.bfloat16 else 0.0)
+                near(got[b, h][fine], want[fine], (rel * size + half_step(dtype) * want.abs())[fine], f"{what} {b} {h}")
+
+    check("large")
+    for b, (page, slot, m) in enumerate(seen):
+        j = int(m.nonzero()[len(lens) - 1 if int(m.sum()) > len(lens) else 0])
+        pool.v[page[j], :, slot[j], b] = float("inf")
+    check("one infinity")
